@@ -87,6 +87,57 @@ class EhipQuantJob(ctypes.Structure):
 
 
 assert ctypes.sizeof(EhipQuantJob) == 32
+
+KV_F32, KV_F16, KV_Q4 = 0, 1, 2
+ROPE_PLAIN, ROPE_LINEAR, ROPE_NTK, ROPE_YARN, ROPE_BANDS = 0, 1, 2, 3, 4
+
+
+class EhipRopeConfig(ctypes.Structure):
+    """ehip.h EhipRopeConfig: how a model's rotary angles are scaled."""
+    _fields_ = [("style", ctypes.c_int32), ("rotary_dim", ctypes.c_int32), ("scaling", ctypes.c_int32),
+                ("orig_ctx", ctypes.c_int32), ("theta", ctypes.c_float), ("factor", ctypes.c_float),
+                ("low", ctypes.c_float), ("high", ctypes.c_float), ("magnitude", ctypes.c_float)]
+
+
+class EhipRopePlan(ctypes.Structure):
+    """ehip.h EhipRopePlan, filled by ehip_rope_plan."""
+    _fields_ = [("style", ctypes.c_int32), ("head_dim", ctypes.c_int32), ("rotary_dim", ctypes.c_int32),
+                ("magnitude", ctypes.c_float), ("turns", ctypes.c_uint64 * 128)]
+
+
+class EhipRopeRows(ctypes.Structure):
+    """ehip.h EhipRopeRows: q|k rows and their positions (device pointers)."""
+    _fields_ = [("x", ctypes.c_void_p), ("out", ctypes.c_void_p), ("x_stride", ctypes.c_int64),
+                ("out_stride", ctypes.c_int64), ("n_tok", ctypes.c_int32), ("n_q", ctypes.c_int32),
+                ("n_k", ctypes.c_int32), ("pos0", ctypes.c_int32), ("pos", ctypes.c_void_p),
+                ("q_norm", ctypes.c_void_p), ("k_norm", ctypes.c_void_p), ("eps", ctypes.c_float)]
+
+
+class EhipCache(ctypes.Structure):
+    """ehip.h EhipCache: one layer's keys and values (device pointers)."""
+    _fields_ = [("k", ctypes.c_void_p), ("v", ctypes.c_void_p), ("ctx", ctypes.c_int64), ("type", ctypes.c_int32),
+                ("n_kv", ctypes.c_int32), ("head_dim", ctypes.c_int32), ("reserved", ctypes.c_int32)]
+
+
+class EhipCacheRows(ctypes.Structure):
+    """ehip.h EhipCacheRows: fp32 rows to be stored (device pointers)."""
+    _fields_ = [("k", ctypes.c_void_p), ("v", ctypes.c_void_p), ("k_stride", ctypes.c_int64),
+                ("v_stride", ctypes.c_int64), ("n_tok", ctypes.c_int32), ("pos0", ctypes.c_int32),
+                ("pos", ctypes.c_void_p)]
+
+
+class EhipAttend(ctypes.Structure):
+    """ehip.h EhipAttend: one attention call (device pointers)."""
+    _fields_ = [("q", ctypes.c_void_p), ("out", ctypes.c_void_p), ("q_stride", ctypes.c_int64),
+                ("out_stride", ctypes.c_int64), ("n_tok", ctypes.c_int32), ("n_heads", ctypes.c_int32),
+                ("pos0", ctypes.c_int32), ("window", ctypes.c_int32), ("sinks", ctypes.c_int32),
+                ("scale", ctypes.c_float), ("pos", ctypes.c_void_p), ("workspace", ctypes.c_void_p),
+                ("workspace_bytes", ctypes.c_uint64)]
+
+
+assert ctypes.sizeof(EhipRopeConfig) == 36 and ctypes.sizeof(EhipRopePlan) == 1040
+assert ctypes.sizeof(EhipRopeRows) == 80 and ctypes.sizeof(EhipCache) == 40
+assert ctypes.sizeof(EhipCacheRows) == 48 and ctypes.sizeof(EhipAttend) == 80
 _FP = ctypes.POINTER(ctypes.c_float)
 _IP = ctypes.POINTER(ctypes.c_int)
 
@@ -151,6 +202,14 @@ PROTOTYPES = {
     "ehip_sample_noalloc": (ctypes.c_int, [_P, ctypes.c_int, ctypes.POINTER(EmberSampler), _P, _P, _P, _P, _P]),
     "ehip_noalloc_setup": (ctypes.c_int, []),
     "ehip_quantize_rows": (ctypes.c_int, [ctypes.POINTER(EhipQuantJob), ctypes.c_int]),
+    "ehip_rope_plan": (ctypes.c_int, [ctypes.POINTER(EhipRopeConfig), ctypes.c_int, ctypes.POINTER(EhipRopePlan)]),
+    "ehip_rope_rows": (ctypes.c_int, [ctypes.POINTER(EhipRopePlan), ctypes.POINTER(EhipRopeRows), _P]),
+    "ehip_cache_bytes": (ctypes.c_uint64, [ctypes.POINTER(EhipCache)]),
+    "ehip_cache_store": (ctypes.c_int, [ctypes.POINTER(EhipCache), ctypes.POINTER(EhipCacheRows), _P]),
+    "ehip_cache_load": (ctypes.c_int, [ctypes.POINTER(EhipCache), ctypes.c_int, ctypes.c_int64, ctypes.c_int, _P,
+                                       ctypes.c_int64, _P]),
+    "ehip_attend_workspace": (ctypes.c_uint64, [ctypes.POINTER(EhipCache), ctypes.c_int, ctypes.c_int]),
+    "ehip_attend": (ctypes.c_int, [ctypes.POINTER(EhipCache), ctypes.POINTER(EhipAttend), _P]),
     # ember_synth.h
     "ember_synth_write": (ctypes.c_int, [ctypes.c_char_p, ctypes.POINTER(EmberSynthConfig)]),
     "ember_synth_fill_row": (None, [ctypes.c_uint64, ctypes.c_char_p, ctypes.c_int, ctypes.c_float,

@@ -1,0 +1,871 @@
+// attend.hip — attention over a device cache of fp32, fp16 or 4 bits, with a
+// sliding window and first positions that stay visible: ehip_attend.
+//
+// For a row (token at position p, query head) of key head g:
+//   s_t = q . k_t * scale,  w_t = exp(s_t - max s),  o = sum w_t v_t / sum w_t
+// over t <= p and, with a window W, t > p - W or t < sinks.  One pass over the
+// cache with a running maximum and sum.
+//
+// A wave takes up to 16 CT rows of one key head (rows are (token, head) pairs,
+// so a cached row serves all its query heads) and tiles of 32 positions:
+//   S^T = K . Q^T  per 16 positions x 16 rows: a lane (l, g) = (lane % 16,
+//         lane / 16) supplies position l of K and row l of Q, 8 dims of quarter
+//         g of every 32, and receives S[position 4g + i][row l], i < 4;
+//   O^T += V^T . P^T  per 16 dims x 16 rows: the contraction runs over the
+//         tile's positions in the order 16s + 4g + i in which the lanes hold
+//         the scores, so a lane's own probabilities are the operand and never
+//         leave its registers, and it receives O[dim 4g + i][row l].
+// The 4-bit cache lies in memory as the lanes use it (EhipCache): a lane's
+// codes come in 16-byte loads, no LDS is passed, and no wave waits for another
+// until the end.
+//
+// Precision.  The fp16 matrix cores take fp32 operands as hi + lo: x scaled by
+// a power of two, hi = fp16(x), lo = fp16(x - hi), |x - hi - lo| <= 2^-23 |x|;
+// products and sums are fp32.  q is scaled per row (its largest element into
+// [2^13, 2^14)), times scale * log2(e) first, so the scores are in log2 units.
+// Codes are exact in fp16; a score is the sum over its blocks of (block's
+// product) * d in fp32.  For P.V each block's scale goes into the
+// probability: w_t d_t, times 2^E with E from the largest |d| so far, keeps
+// both halves in fp16's range (below 2^15: what a half loses at its smallest
+// is 2^-38 of the largest).  The outputs' sums carry 2^E until the end.  An
+// fp16 cache is exact already and has E = 14; an fp32 cache goes through the
+// fp32 matrix cores as it is, with E = 0.
+//
+// What a row does not see cannot reach it: its scores are selected away, its
+// probabilities are zero, and where a zero times what the cache holds would be
+// NaN (infinite or NaN values, scales of positions never stored) the factor is
+// selected away too (4 bits: the scale) or the value's products are made one
+// by one for the rows that see it.
+#include "session.h"
+
+namespace ehip {
+
+typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
+typedef unsigned short u16x2 __attribute__((ext_vector_type(2)));
+typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
+
+struct AttendArgs {
+    const float *q;
+    float *out;
+    int64_t q_stride, out_stride;
+    const uint8_t *kc, *vc;
+    int64_t head_bytes;          // 4 bits: bytes of a key head's tiles
+    int kvd;                     // others: elements of a position
+    int n_tok, n_kv, G, pos0, ctx;
+    const int *pos;
+    int out_vec;                 // out rows take 16-byte stores
+    int window, sinks;
+    float qscale;                // scale * log2(e)
+    int nsplit;                  // workgroups that share a row group's positions
+    float *part;                 // [unit][nsplit][rows][HD], then float4 [unit][nsplit][rows]; unit = (row group, key head)
+    float4 *part_ml;             // a row's maximum, sum and score scale
+    int *count;                  // [unit]: workgroups of the unit that are done; zero between launches
+};
+
+constexpr int AT_WAVES = 4;      // waves of a workgroup: they share its rows and take tiles in turn
+
+// maximum / sum over the four lane quarters of a row
+__device__ __forceinline__ float quarters_max(float v) {
+    const auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    v = fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1]));
+    const auto t = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    return fmaxf(__uint_as_float(t[0]), __uint_as_float(t[1]));
+}
+__device__ __forceinline__ float quarters_sum(float v) { return xor32_add(xor16_add(v)); }
+
+__device__ __forceinline__ uint32_t pack2(_Float16 a, _Float16 b) {
+    return (uint32_t)__builtin_bit_cast(uint16_t, a) | ((uint32_t)__builtin_bit_cast(uint16_t, b) << 16);
+}
+__device__ __forceinline__ f16x8 as_f16(i32x4 v) { return __builtin_bit_cast(f16x8, v); }
+// fp16 number in half s of a dword, widened
+__device__ __forceinline__ float half_of(int w, int s) { return (float)__builtin_bit_cast(f16x2, w)[s]; }
+
+// The 8 codes of a dword, minus 8, as fp16 pairs (n, n + 4), n = 0 .. 3; the
+// pairs of odd n come 16 times too large, which their partner operand makes
+// up.  0x6400 is 1024, whose last mantissa bits take a code as it lies (the low
+// nibble) or 16 times it.
+__device__ __forceinline__ i32x4 codes_signed(uint32_t w) {
+    const f16x2 lo = { (_Float16)-1032.0f, (_Float16)-1032.0f }, hi = { (_Float16)-1152.0f, (_Float16)-1152.0f };
+    auto one = [](uint32_t bits, f16x2 off) { return __builtin_bit_cast(int, __builtin_bit_cast(f16x2, bits) + off); };
+    const uint32_t v = w >> 8;
+    return i32x4{ one((w & 0x000f000fu) | 0x64006400u, lo), one((w & 0x00f000f0u) | 0x64006400u, hi),
+                  one((v & 0x000f000fu) | 0x64006400u, lo), one((v & 0x00f000f0u) | 0x64006400u, hi) };
+}
+
+// Which tiles of 32 positions the rows r0 .. r1 - 1 of a launch see: the sinks'
+// tiles [0, ns), then those from w0 on; n in all, tile of index v.
+struct Tiles {
+    int ns, w0, n;
+    __device__ __forceinline__ int at(int v) const { return v < ns ? v : v - ns + w0; }
+};
+__device__ __forceinline__ Tiles tiles_seen(int first_pos, int last_pos, int window, int sinks) {
+    Tiles t;
+    const int last = last_pos / KV_TILE;
+    t.ns = 0;
+    t.w0 = 0;
+    if (window > 0) {
+        t.ns = sinks > 0 ? min((sinks - 1) / KV_TILE, last) + 1 : 0;
+        t.w0 = max(max(first_pos - window + 1, 0) / KV_TILE, t.ns);
+    }
+    t.n = t.ns + max(last + 1 - t.w0, 0);
+    return t;
+}
+
+// The rows of a wave: CT groups of 16 (PACK: one of 8, whose columns 8 .. 15
+// hold the low halves of the same rows), their running softmax and output.
+template <int HD, int CT> struct Rows {
+    float sc[CT];                // score = product * sc
+    int p[CT];                   // the row's position
+    float m[CT], l[CT];          // maximum (in products), this lane's share of the sum
+    f32x4 o[CT][HD / 16];
+};
+
+// sum and maximum updates shared by the cache types: S[c][s][i] are products
+// (masked ones -inf), which become the probabilities 2^((S - max) sc).  up: what
+// the output's sums are multiplied by beside (a new exponent), 1 mostly.
+template <int HD, int CT>
+__device__ __forceinline__ void softmax_step(Rows<HD, CT> &R, f32x4 (&S)[CT][2], float up) {
+#pragma unroll
+    for (int c = 0; c < CT; c++) {
+        float t = fmaxf(fmaxf(S[c][0][0], S[c][0][1]), fmaxf(S[c][0][2], S[c][0][3]));
+        t = fmaxf(t, fmaxf(fmaxf(S[c][1][0], S[c][1][1]), fmaxf(S[c][1][2], S[c][1][3])));
+        const float mn = fmaxf(R.m[c], quarters_max(t));
+        if (__any(mn > R.m[c]) || up != 1.0f) {
+            const float a = R.m[c] == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f((R.m[c] - mn) * R.sc[c]);
+            R.l[c] *= a;
+#pragma unroll
+            for (int d = 0; d < HD / 16; d++) R.o[c][d] *= a * up;
+            R.m[c] = mn;
+        }
+        // (the difference first: the exponential's argument is then off by
+        // its own rounding only, at whatever size the scores are)
+        const float mu = mn == -INFINITY ? 0.0f : mn;
+        float l = 0.0f;
+#pragma unroll
+        for (int s = 0; s < 2; s++)
+#pragma unroll
+            for (int i = 0; i < 4; i++) {
+                S[c][s][i] = __builtin_amdgcn_exp2f((S[c][s][i] - mu) * R.sc[c]);
+                l += S[c][s][i];
+            }
+        R.l[c] += l;
+    }
+}
+
+// the scores of positions that a row does not see become -inf
+template <int HD, int CT>
+__device__ __forceinline__ bool seen(const AttendArgs &a, const Rows<HD, CT> &R, int c, int t) {
+    return t <= R.p[c] && (a.window <= 0 || t > R.p[c] - a.window || t < a.sinks);
+}
+template <int HD, int CT>
+__device__ __forceinline__ void mask_scores(const AttendArgs &a, const Rows<HD, CT> &R, f32x4 (&S)[CT][2], int t0) {
+    const int g = (threadIdx.x & 63) >> 4;
+#pragma unroll
+    for (int c = 0; c < CT; c++)
+#pragma unroll
+        for (int s = 0; s < 2; s++)
+#pragma unroll
+            for (int i = 0; i < 4; i++)
+                if (!seen(a, R, c, t0 + 16 * s + 4 * g + i)) S[c][s][i] = -INFINITY;
+}
+
+// ---- one tile of each cache type ------------------------------------------
+// The Q operand of the fp16 matrix cores: q[c][b][0] the high halves, [1] the
+// low ones (PACK: [0] alone, high or low by the column).
+template <int HD, int CT, bool PACK> struct QHalf {
+    static constexpr int NB = (HD + 31) / 32, NH = PACK ? 1 : 2;
+    i32x4 q[CT][NB][NH];
+};
+
+// Loads a row's dims 32 b + 8 g .. + 7, scales and splits them.  ORDER4: the
+// element order of a code dword, (0, 4), (1, 5) / 16, (2, 6), (3, 7) / 16.
+template <int HD, int CT, bool PACK, bool ORDER4>
+__device__ __forceinline__ void load_q16(const AttendArgs &a, const float *row, int c, QHalf<HD, CT, PACK> &Q, float &sc) {
+    constexpr int NB = QHalf<HD, CT, PACK>::NB;
+    const int lane = threadIdx.x & 63, g = lane >> 4;
+    float x[NB][8];
+    float top = 0.0f;
+#pragma unroll
+    for (int b = 0; b < NB; b++)
+#pragma unroll
+        for (int j = 0; j < 8; j++) {
+            const int d = 32 * b + 8 * g + j;
+            x[b][j] = HD % 32 == 0 || d < HD ? row[HD % 32 == 0 ? d : min(d, HD - 1)] * a.qscale : 0.0f;
+            top = fmaxf(top, fabsf(x[b][j]));
+        }
+    top = quarters_max(top);
+    const int e = top > 0.0f ? 14 - __builtin_amdgcn_frexp_expf(top) : 0;   // top 2^e in [2^13, 2^14)
+    sc = __builtin_amdgcn_ldexpf(1.0f, -e);
+#pragma unroll
+    for (int b = 0; b < NB; b++) {
+        _Float16 hi[8], lo[8];
+#pragma unroll
+        for (int j = 0; j < 8; j++) {
+            const float y = __builtin_amdgcn_ldexpf(x[b][j], ORDER4 && (j & 1) ? e - 4 : e);
+            hi[j] = (_Float16)y;
+            lo[j] = (_Float16)(y - (float)hi[j]);
+        }
+        i32x4 h, w;
+        if (ORDER4) {
+            h = i32x4{ (int)pack2(hi[0], hi[4]), (int)pack2(hi[1], hi[5]), (int)pack2(hi[2], hi[6]), (int)pack2(hi[3], hi[7]) };
+            w = i32x4{ (int)pack2(lo[0], lo[4]), (int)pack2(lo[1], lo[5]), (int)pack2(lo[2], lo[6]), (int)pack2(lo[3], lo[7]) };
+        } else {
+            h = i32x4{ (int)pack2(hi[0], hi[1]), (int)pack2(hi[2], hi[3]), (int)pack2(hi[4], hi[5]), (int)pack2(hi[6], hi[7]) };
+            w = i32x4{ (int)pack2(lo[0], lo[1]), (int)pack2(lo[2], lo[3]), (int)pack2(lo[4], lo[5]), (int)pack2(lo[6], lo[7]) };
+        }
+        if (PACK) Q.q[c][b][0] = (lane & 8) ? w : h;
+        else { Q.q[c][b][0] = h; Q.q[c][b][QHalf<HD, CT, PACK>::NH - 1] = w; }
+    }
+}
+
+__device__ __forceinline__ f32x4 mfma16(i32x4 a, i32x4 b, f32x4 c) {
+    return __builtin_amdgcn_mfma_f32_16x16x32_f16(as_f16(a), as_f16(b), c, 0, 0, 0);
+}
+
+// rows 0 .. 7 and their low halves in columns 8 .. 15, added in both
+__device__ __forceinline__ f32x4 add_halves(f32x4 v) {
+#pragma unroll
+    for (int i = 0; i < 4; i++) v[i] = xor8_add(v[i]);
+    return v;
+}
+
+// The hi and lo halves of 8 probabilities w[s][i] as the P operand: pairs
+// (s = 0, s = 1) of i.
+template <bool PACK>
+__device__ __forceinline__ void split_p(const float (&w)[2][4], i32x4 &hi, i32x4 &lo) {
+    const bool low = PACK && ((threadIdx.x & 8) != 0);
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+        const _Float16 a = (_Float16)w[0][i], b = (_Float16)w[1][i];
+        const _Float16 la = (_Float16)(w[0][i] - (float)a), lb = (_Float16)(w[1][i] - (float)b);
+        if (PACK) {
+            hi[i] = (int)(low ? pack2(la, lb) : pack2(a, b));
+        } else {
+            hi[i] = (int)pack2(a, b);
+            lo[i] = (int)pack2(la, lb);
+        }
+    }
+}
+
+template <int TYPE, int HD, int CT, bool PACK> struct Tile;
+
+// 4 bits: HD / 16 dwords of codes for keys and for values per lane, and the
+// scales of the lane's 8 positions (dword b * 4 + i: positions s = 0, 1)
+template <int HD, int CT, bool PACK> struct Tile<EHIP_KV_Q4, HD, CT, PACK> {
+    static constexpr int NB = HD / QB, NP = HD / 64;
+    i32x4 k[NP], v[NP], ks[NB], vs[NB];
+    QHalf<HD, CT, PACK> Q;
+    int top = 0x0400;            // the largest |d| of a value so far (fp16 bits), at least 2^-14
+    int E = 29 - (0x0400 >> 10);   // |d| < 2^((top >> 10) - 14): the factors stay below 2^15
+    const uint8_t *kb, *vb;
+
+    __device__ __forceinline__ void init(const AttendArgs &a, int kv) {
+        const int lane = threadIdx.x & 63;
+        kb = a.kc + kv * a.head_bytes;
+        vb = a.vc + kv * a.head_bytes;
+        (void)lane;
+    }
+    __device__ __forceinline__ void load_q(const AttendArgs &a, const float *row, int c, float &sc) {
+        load_q16<HD, CT, PACK, true>(a, row, c, Q, sc);
+    }
+    __device__ __forceinline__ void load_k(const AttendArgs &, int tile, int) {
+        const int lane = threadIdx.x & 63, g = lane >> 4;
+        const uint8_t *t = kb + (int64_t)tile * kv_tile_bytes(HD);
+#pragma unroll
+        for (int i = 0; i < NP; i++) k[i] = *reinterpret_cast<const i32x4 *>(t + i * 1024 + lane * 16);
+#pragma unroll
+        for (int b = 0; b < NB; b++) ks[b] = *reinterpret_cast<const i32x4 *>(t + kv_scale_at(HD, g, b, 0, 0));
+    }
+    __device__ __forceinline__ void load_v(const AttendArgs &, int tile, int) {
+        const int lane = threadIdx.x & 63, g = lane >> 4;
+        const uint8_t *t = vb + (int64_t)tile * kv_tile_bytes(HD);
+#pragma unroll
+        for (int i = 0; i < NP; i++) v[i] = *reinterpret_cast<const i32x4 *>(t + i * 1024 + lane * 16);
+#pragma unroll
+        for (int b = 0; b < NB; b++) vs[b] = *reinterpret_cast<const i32x4 *>(t + kv_scale_at(HD, g, b, 0, 0));
+    }
+    __device__ __forceinline__ void scores(f32x4 (&S)[CT][2]) {
+#pragma unroll
+        for (int s = 0; s < 2; s++) {
+#pragma unroll
+            for (int c = 0; c < CT; c++) S[c][s] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+            for (int b = 0; b < NB; b++) {
+                const int e = s * NB + b;
+                const i32x4 codes = codes_signed((uint32_t)k[e >> 2][e & 3]);
+#pragma unroll
+                for (int c = 0; c < CT; c++) {
+                    f32x4 x = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+                    for (int h = 0; h < QHalf<HD, CT, PACK>::NH; h++) x = mfma16(codes, Q.q[c][b][h], x);
+#pragma unroll
+                    for (int i = 0; i < 4; i++) S[c][s][i] = __builtin_fmaf(x[i], half_of(ks[b][i], s), S[c][s][i]);
+                }
+            }
+            if (PACK) S[0][s] = add_halves(S[0][s]);
+        }
+    }
+    // masked: t0 the tile's first position, lo_seen / hi_seen the positions that any row sees
+    template <bool MASKED>
+    __device__ __forceinline__ void values(const AttendArgs &a, Rows<HD, CT> &R, f32x4 (&S)[CT][2], int t0, int kv, int first_pos, int last_pos) {
+        const int g = (threadIdx.x & 63) >> 4;
+        // the largest finite |d| among the positions that a row sees
+        u16x2 mx = { 0, 0 };
+#pragma unroll
+        for (int b = 0; b < NB; b++)
+#pragma unroll
+            for (int i = 0; i < 4; i++) {
+                u16x2 w = __builtin_bit_cast(u16x2, vs[b][i] & 0x7fff7fff);
+                if (MASKED) {
+#pragma unroll
+                    for (int s = 0; s < 2; s++) {
+                        const int t = t0 + 16 * s + 4 * g + i;
+                        if (!(t <= last_pos && (a.window <= 0 || t > first_pos - a.window || t < a.sinks))) w[s] = 0;
+                    }
+                }
+                mx = __builtin_elementwise_max(mx, w);
+            }
+        int big = max((int)mx[0], (int)mx[1]);
+        if (__any(big >= 0x7c00)) {   // the block of a NaN: its rows' sums are NaN at any E
+            big = 0;
+#pragma unroll
+            for (int b = 0; b < NB; b++)
+#pragma unroll
+                for (int i = 0; i < 4; i++)
+#pragma unroll
+                    for (int s = 0; s < 2; s++) {
+                        const int t = t0 + 16 * s + 4 * g + i, w = vs[b][i] >> (16 * s) & 0x7fff;
+                        if (w < 0x7c00 && t <= last_pos && (a.window <= 0 || t > first_pos - a.window || t < a.sinks)) big = max(big, w);
+                    }
+        }
+        big = max(big, __shfl_xor(big, 16));
+        big = max(big, __shfl_xor(big, 32));
+        top = max(top, big);
+        const int En = 29 - (top >> 10);
+        softmax_step(R, S, __builtin_amdgcn_ldexpf(1.0f, En - E));
+        E = En;
+        const float even = __builtin_amdgcn_ldexpf(1.0f, E), odd = even * 0.0625f;   // (the codes of odd i are 16 times too large)
+#pragma unroll
+        for (int c = 0; c < CT; c++)
+#pragma unroll
+            for (int s = 0; s < 2; s++)
+#pragma unroll
+                for (int i = 0; i < 4; i++) S[c][s][i] *= i & 1 ? odd : even;
+#pragma unroll
+        for (int b = 0; b < NB; b++) {
+            const i32x4 c0 = codes_signed((uint32_t)v[(2 * b) >> 2][(2 * b) & 3]), c1 = codes_signed((uint32_t)v[(2 * b + 1) >> 2][(2 * b + 1) & 3]);
+#pragma unroll
+            for (int c = 0; c < CT; c++) {
+                float w[2][4];
+#pragma unroll
+                for (int s = 0; s < 2; s++)
+#pragma unroll
+                    for (int i = 0; i < 4; i++) {
+                        w[s][i] = S[c][s][i] * half_of(vs[b][i], s);
+                        if (MASKED && !seen(a, R, c, t0 + 16 * s + 4 * g + i)) w[s][i] = 0.0f;
+                    }
+                i32x4 hi, lo;
+                split_p<PACK>(w, hi, lo);
+                R.o[c][2 * b] = mfma16(c0, hi, R.o[c][2 * b]);
+                R.o[c][2 * b + 1] = mfma16(c1, hi, R.o[c][2 * b + 1]);
+                if (!PACK) {
+                    R.o[c][2 * b] = mfma16(c0, lo, R.o[c][2 * b]);
+                    R.o[c][2 * b + 1] = mfma16(c1, lo, R.o[c][2 * b + 1]);
+                }
+            }
+        }
+        (void)kv;
+    }
+    __device__ __forceinline__ int exponent() const { return E; }
+};
+
+// The values of a masked tile that are not finite, for the rows that see
+// them, one position at a time: o[dim][row] += p v (the tile's products took
+// them as zero).  P: the probabilities.
+template <int HD, int CT, bool F16, bool PACK>
+__device__ __forceinline__ void odd_values(const AttendArgs &a, Rows<HD, CT> &R, f32x4 (&P)[CT][2], int t0, int kv, int last_pos) {
+    const int lane = threadIdx.x & 63, g = lane >> 4, l = lane & 15;
+    const bool low = PACK && (lane & 8);
+#pragma unroll 1
+    for (int h = 0; h < 4; h++)
+#pragma unroll
+        for (int s = 0; s < 2; s++)
+#pragma unroll
+            for (int i = 0; i < 4; i++) {
+                const int t = t0 + 16 * s + 4 * h + i;
+                const int64_t at = (int64_t)min(t, last_pos) * a.kvd + kv * HD;
+#pragma unroll
+                for (int c = 0; c < CT; c++) {
+                    const float p = __shfl(P[c][s][i], h * 16 + l);
+                    const bool in = seen(a, R, c, t) && !low;
+#pragma unroll
+                    for (int d = 0; d < HD / 16; d++)
+#pragma unroll
+                        for (int r = 0; r < 4; r++) {
+                            const int64_t e = at + 16 * d + 4 * g + r;
+                            const float v = F16 ? (float)reinterpret_cast<const _Float16 *>(a.vc)[e] : reinterpret_cast<const float *>(a.vc)[e];
+                            if (in && !(fabsf(v) < INFINITY)) R.o[c][d][r] += p * v;   // (not finite: 2^E does not matter)
+                        }
+                }
+            }
+}
+
+// fp16: the lanes' pieces of K are 16-byte loads; a V operand is gathered from
+// 8 positions (64 bytes of a position to 16 lanes).  Positions past last_pos
+// repeat it.
+template <int HD, int CT, bool PACK> struct Tile<EHIP_KV_F16, HD, CT, PACK> {
+    static constexpr int NB = (HD + 31) / 32;
+    i32x4 k[2][NB], v[HD / 16];
+    QHalf<HD, CT, PACK> Q;
+    const _Float16 *kb, *vb;
+
+    __device__ __forceinline__ void init(const AttendArgs &a, int kv) {
+        kb = reinterpret_cast<const _Float16 *>(a.kc) + kv * HD;
+        vb = reinterpret_cast<const _Float16 *>(a.vc) + kv * HD;
+    }
+    __device__ __forceinline__ void load_q(const AttendArgs &a, const float *row, int c, float &sc) {
+        load_q16<HD, CT, PACK, false>(a, row, c, Q, sc);
+    }
+    __device__ __forceinline__ void load_k(const AttendArgs &a, int tile, int last_pos) {
+        const int lane = threadIdx.x & 63, g = lane >> 4;
+#pragma unroll
+        for (int s = 0; s < 2; s++) {
+            const _Float16 *r = kb + (int64_t)min(tile * KV_TILE + 16 * s + (lane & 15), last_pos) * a.kvd;
+#pragma unroll
+            for (int b = 0; b < NB; b++) {
+                const bool in = HD % 32 == 0 || 32 * b + 8 * g < HD;   // (HD 48: the last piece's upper half is zero)
+                k[s][b] = *reinterpret_cast<const i32x4 *>(r + (in ? 32 * b + 8 * g : 0));
+                if (!in) k[s][b] = i32x4{0, 0, 0, 0};
+            }
+        }
+    }
+    __device__ __forceinline__ void load_v(const AttendArgs &a, int tile, int last_pos) {
+        const int lane = threadIdx.x & 63, g = lane >> 4;
+        const uint16_t *base = reinterpret_cast<const uint16_t *>(vb) + (lane & 15);
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+            const int t = tile * KV_TILE + 4 * g + i;
+            const uint16_t *r0 = base + (int64_t)min(t, last_pos) * a.kvd, *r1 = base + (int64_t)min(t + 16, last_pos) * a.kvd;
+#pragma unroll
+            for (int d = 0; d < HD / 16; d++) v[d][i] = (int)((uint32_t)r0[16 * d] | ((uint32_t)r1[16 * d] << 16));
+        }
+    }
+    __device__ __forceinline__ void scores(f32x4 (&S)[CT][2]) {
+#pragma unroll
+        for (int s = 0; s < 2; s++)
+#pragma unroll
+            for (int c = 0; c < CT; c++) {
+                S[c][s] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+                for (int b = 0; b < NB; b++)
+#pragma unroll
+                    for (int h = 0; h < QHalf<HD, CT, PACK>::NH; h++) S[c][s] = mfma16(k[s][b], Q.q[c][b][h], S[c][s]);
+                if (PACK) S[c][s] = add_halves(S[c][s]);
+            }
+    }
+    template <bool MASKED>
+    __device__ __forceinline__ void values(const AttendArgs &a, Rows<HD, CT> &R, f32x4 (&S)[CT][2], int t0, int kv, int, int last_pos) {
+        bool odd = false;
+        if (MASKED) {   // what is not finite goes to its own rows only
+#pragma unroll
+            for (int d = 0; d < HD / 16; d++)
+#pragma unroll
+                for (int i = 0; i < 4; i++) {
+                    const bool a0 = (v[d][i] & 0x7c00) == 0x7c00, a1 = (v[d][i] & 0x7c000000) == 0x7c000000;
+                    odd |= a0 | a1;
+                    if (a0) v[d][i] &= (int)0xffff0000;
+                    if (a1) v[d][i] &= 0x0000ffff;
+                }
+        }
+        softmax_step(R, S, 1.0f);
+#pragma unroll
+        for (int c = 0; c < CT; c++) {
+            float w[2][4];
+#pragma unroll
+            for (int s = 0; s < 2; s++)
+#pragma unroll
+                for (int i = 0; i < 4; i++) w[s][i] = S[c][s][i] * 16384.0f;
+            i32x4 hi, lo;
+            split_p<PACK>(w, hi, lo);
+#pragma unroll
+            for (int d = 0; d < HD / 16; d++) {
+                R.o[c][d] = mfma16(v[d], hi, R.o[c][d]);
+                if (!PACK) R.o[c][d] = mfma16(v[d], lo, R.o[c][d]);
+            }
+        }
+        if (MASKED && __any(odd)) odd_values<HD, CT, true, PACK>(a, R, S, t0, kv, last_pos);
+    }
+    __device__ __forceinline__ int exponent() const { return 14; }
+};
+
+// fp32, on the fp32 matrix cores (16x16x4): lane quarter g supplies dims
+// g HD / 4 .. of K and Q, so its pieces are contiguous; a P.V step contracts
+// one position per quarter.
+template <int HD, int CT, bool PACK> struct Tile<EHIP_KV_F32, HD, CT, PACK> {
+    static_assert(!PACK, "fp32 rows have no low halves");
+    static constexpr int NQ = HD / 16;   // 16-byte pieces of a quarter
+    f32x4 k[2][NQ], q[CT][NQ];
+    float v[HD / 16][2][4];
+    const float *kb, *vb;
+
+    __device__ __forceinline__ void init(const AttendArgs &a, int kv) {
+        kb = reinterpret_cast<const float *>(a.kc) + kv * HD;
+        vb = reinterpret_cast<const float *>(a.vc) + kv * HD;
+    }
+    __device__ __forceinline__ void load_q(const AttendArgs &a, const float *row, int c, float &sc) {
+        const int g = (threadIdx.x & 63) >> 4;
+#pragma unroll
+        for (int j = 0; j < NQ; j++)
+#pragma unroll
+            for (int r = 0; r < 4; r++) q[c][j][r] = row[g * (HD / 4) + 4 * j + r] * a.qscale;
+        sc = 1.0f;
+    }
+    __device__ __forceinline__ void load_k(const AttendArgs &a, int tile, int last_pos) {
+        const int lane = threadIdx.x & 63, g = lane >> 4;
+#pragma unroll
+        for (int s = 0; s < 2; s++) {
+            const float *r = kb + (int64_t)min(tile * KV_TILE + 16 * s + (lane & 15), last_pos) * a.kvd + g * (HD / 4);
+#pragma unroll
+            for (int j = 0; j < NQ; j++) k[s][j] = *reinterpret_cast<const f32x4 *>(r + 4 * j);
+        }
+    }
+    __device__ __forceinline__ void load_v(const AttendArgs &a, int tile, int last_pos) {
+        const int lane = threadIdx.x & 63, g = lane >> 4;
+#pragma unroll
+        for (int s = 0; s < 2; s++)
+#pragma unroll
+            for (int i = 0; i < 4; i++) {
+                const float *r = vb + (int64_t)min(tile * KV_TILE + 16 * s + 4 * g + i, last_pos) * a.kvd + (lane & 15);
+#pragma unroll
+                for (int d = 0; d < HD / 16; d++) v[d][s][i] = r[16 * d];
+            }
+    }
+    __device__ __forceinline__ void scores(f32x4 (&S)[CT][2]) {
+#pragma unroll
+        for (int s = 0; s < 2; s++)
+#pragma unroll
+            for (int c = 0; c < CT; c++) {
+                S[c][s] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+                for (int j = 0; j < NQ; j++)
+#pragma unroll
+                    for (int r = 0; r < 4; r++) S[c][s] = __builtin_amdgcn_mfma_f32_16x16x4f32(k[s][j][r], q[c][j][r], S[c][s], 0, 0, 0);
+            }
+    }
+    template <bool MASKED>
+    __device__ __forceinline__ void values(const AttendArgs &a, Rows<HD, CT> &R, f32x4 (&S)[CT][2], int t0, int kv, int, int last_pos) {
+        bool odd = false;
+        if (MASKED) {
+#pragma unroll
+            for (int d = 0; d < HD / 16; d++)
+#pragma unroll
+                for (int s = 0; s < 2; s++)
+#pragma unroll
+                    for (int i = 0; i < 4; i++) {
+                        const bool bad = !(fabsf(v[d][s][i]) < INFINITY);
+                        odd |= bad;
+                        if (bad) v[d][s][i] = 0.0f;
+                    }
+        }
+        softmax_step(R, S, 1.0f);
+#pragma unroll
+        for (int c = 0; c < CT; c++)
+#pragma unroll
+            for (int d = 0; d < HD / 16; d++)
+#pragma unroll
+                for (int s = 0; s < 2; s++)
+#pragma unroll
+                    for (int i = 0; i < 4; i++) R.o[c][d] = __builtin_amdgcn_mfma_f32_16x16x4f32(v[d][s][i], S[c][s][i], R.o[c][d], 0, 0, 0);
+        if (MASKED && __any(odd)) odd_values<HD, CT, false, PACK>(a, R, S, t0, kv, last_pos);
+    }
+    __device__ __forceinline__ int exponent() const { return 0; }
+};
+
+// dims d .. d + 3 of row r of key head kv: o / l
+template <int HD>
+__device__ __forceinline__ void store_out(const AttendArgs &a, int pos0, int kv, int r, int d, f32x4 o, float l) {
+    const int b = r / a.G;
+    const float inv = 1.0f / l;
+    o *= inv;
+    if (pos0 + b < 0 || pos0 + b >= a.ctx) o = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+    float *dst = a.out + (int64_t)b * a.out_stride + (kv * a.G + r % a.G) * HD + d;
+    if (a.out_vec) {
+        *reinterpret_cast<f32x4 *>(dst) = o;
+    } else {
+#pragma unroll
+        for (int j = 0; j < 4; j++) dst[j] = o[j];
+    }
+}
+
+// ---- the kernel ------------------------------------------------------------
+// Workgroup (unit, split): unit = (row group, key head), key heads fastest so
+// that a key head's workgroups share an XCD's L2; row groups from the last, so
+// that the longest start first.  The unit's nsplit workgroups take equal runs
+// of its tiles (those without one leave), and the wave w of a workgroup the
+// tiles w, w + 4, ... of the run.  The last workgroup of a unit to arrive puts
+// the runs together.
+template <int TYPE, int HD, int CT, bool PACK>
+__global__ __launch_bounds__(64 * AT_WAVES) void k_attend(AttendArgs a) {
+    constexpr int BR = PACK ? 8 : 16 * CT;        // rows of a unit
+    constexpr int LD = HD + 4;                    // floats between rows in LDS
+    __shared__ __align__(16) float so[AT_WAVES][BR][LD];
+    __shared__ float sm[AT_WAVES][BR], sl[AT_WAVES][BR], ssc[BR], se[AT_WAVES];
+    __shared__ int s_last;
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, g = lane >> 4;
+    const int nunits = gridDim.x / a.nsplit;
+    const int unit = blockIdx.x % nunits, split = blockIdx.x / nunits;
+    const int kv = unit % a.n_kv, groups = nunits / a.n_kv;
+    const int nrows = a.n_tok * a.G, r0 = (groups - 1 - unit / a.n_kv) * BR, r1 = min(r0 + BR, nrows);
+    const int pos0 = a.pos ? max(min(*a.pos, a.ctx), -a.n_tok) : a.pos0;
+    // rows whose position lies outside the cache (a device position only) give zeros
+    const int first_pos = max(pos0 + r0 / a.G, 0), last_pos = min(pos0 + (r1 - 1) / a.G, a.ctx - 1);
+    const Tiles T = tiles_seen(first_pos, last_pos, a.window, a.sinks);
+    const int ntiles = last_pos < first_pos ? 0 : T.n;
+    const int run = max((ntiles + a.nsplit - 1) / a.nsplit, 1), nact = max((ntiles + run - 1) / run, 1);
+    if (split >= nact) return;
+    const int v1 = min((split + 1) * run, ntiles);
+
+    Rows<HD, CT> R;
+    Tile<TYPE, HD, CT, PACK> X;
+    X.init(a, kv);
+    int vi = split * run + wave;
+    if (vi < v1) {
+        X.load_k(a, T.at(vi), last_pos);
+        X.load_v(a, T.at(vi), last_pos);
+    }
+#pragma unroll
+    for (int c = 0; c < CT; c++) {
+        const int r = min(r0 + 16 * c + (lane & (PACK ? 7 : 15)), nrows - 1), b = r / a.G;
+        R.p[c] = pos0 + b;
+        R.m[c] = -INFINITY;
+        R.l[c] = 0.0f;
+#pragma unroll
+        for (int d = 0; d < HD / 16; d++) R.o[c][d] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+        X.load_q(a, a.q + (int64_t)b * a.q_stride + (kv * a.G + r % a.G) * HD, c, R.sc[c]);
+    }
+    // positions that every row sees: up to that of the first row, and from the last row's window on (or a sink)
+    const int all_to = pos0 + r0 / a.G, all_from = a.window > 0 ? pos0 + (r1 - 1) / a.G - a.window + 1 : 0;
+    while (vi < v1) {
+        const int tile = T.at(vi), t0 = tile * KV_TILE;
+        const bool whole = t0 + KV_TILE - 1 <= all_to && (t0 >= all_from || t0 + KV_TILE <= a.sinks);
+        f32x4 S[CT][2];
+        X.scores(S);
+        vi += AT_WAVES;
+        if (vi < v1) X.load_k(a, T.at(vi), last_pos);
+        if (whole) {
+            X.template values<false>(a, R, S, t0, kv, first_pos, last_pos);
+        } else {
+            mask_scores(a, R, S, t0);
+            X.template values<true>(a, R, S, t0, kv, first_pos, last_pos);
+        }
+        if (vi < v1) X.load_v(a, T.at(vi), last_pos);
+    }
+
+    // ---- the workgroup's waves: a row's sums weigh 2^((m - M) sc), M the largest of its m, the output's 2^-E of it
+    const int E = X.exponent();
+#pragma unroll
+    for (int c = 0; c < CT; c++) {
+        const int r = 16 * c + (lane & (PACK ? 7 : 15));
+        const float l = quarters_sum(R.l[c]);
+        if (g == 0 && !(PACK && (lane & 8))) {
+            sm[wave][r] = R.m[c];
+            sl[wave][r] = l;
+            ssc[r] = R.sc[c];   // every wave's is the same
+        }
+#pragma unroll
+        for (int d = 0; d < HD / 16; d++) {
+            f32x4 o = R.o[c][d];
+            if (PACK) o = add_halves(o);
+            if (!(PACK && (lane & 8))) *reinterpret_cast<f32x4 *>(&so[wave][r][16 * d + 4 * g]) = o;
+        }
+    }
+    if (lane == 0) se[wave] = __builtin_amdgcn_ldexpf(1.0f, -E);
+    __syncthreads();
+    const bool alone = nact == 1;
+    const int64_t slot = (int64_t)unit * a.nsplit + split;
+    for (int i = tid; i < BR * (HD / 4); i += 64 * AT_WAVES) {
+        const int r = i / (HD / 4), d = i % (HD / 4) * 4;
+        float M = sm[0][r];
+#pragma unroll
+        for (int w = 1; w < AT_WAVES; w++) M = fmaxf(M, sm[w][r]);
+        f32x4 o = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+        float l = 0.0f;
+#pragma unroll
+        for (int w = 0; w < AT_WAVES; w++) {
+            const float f = sm[w][r] == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f((sm[w][r] - M) * ssc[r]);
+            o += *reinterpret_cast<const f32x4 *>(&so[w][r][d]) * (f * se[w]);
+            l += sl[w][r] * f;
+        }
+        if (r0 + r >= nrows) continue;
+        if (alone) {
+            store_out<HD>(a, pos0, kv, r0 + r, d, o, l);
+        } else {
+            // agent scope: another XCD's workgroup reads them
+            float *p = a.part + (slot * BR + r) * HD + d;
+#pragma unroll
+            for (int j = 0; j < 4; j++) __hip_atomic_store(p + j, o[j], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+            if (d == 0) {
+                __hip_atomic_store(&a.part_ml[slot * BR + r].x, M, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+                __hip_atomic_store(&a.part_ml[slot * BR + r].y, l, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+                __hip_atomic_store(&a.part_ml[slot * BR + r].z, ssc[r], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+            }
+        }
+    }
+    if (alone) return;
+
+    // ---- the unit's workgroups: the last one to arrive joins the runs
+    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "agent");
+    __syncthreads();
+    if (tid == 0) s_last = __hip_atomic_fetch_add(a.count + unit, 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == nact - 1;
+    __syncthreads();
+    if (!s_last) return;
+    __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "agent");
+    if (tid == 0) __hip_atomic_store(a.count + unit, 0, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    const int64_t base = (int64_t)unit * a.nsplit;
+    for (int i = tid; i < (r1 - r0) * (HD / 4); i += 64 * AT_WAVES) {
+        const int r = i / (HD / 4), d = i % (HD / 4) * 4;
+        const float sc = __hip_atomic_load(&a.part_ml[base * BR + r].z, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+        float M = -INFINITY;
+        for (int z = 0; z < nact; z++) M = fmaxf(M, __hip_atomic_load(&a.part_ml[(base + z) * BR + r].x, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT));
+        f32x4 o = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+        float l = 0.0f;
+        for (int z = 0; z < nact; z++) {
+            const float m = __hip_atomic_load(&a.part_ml[(base + z) * BR + r].x, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+            const float f = m == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f((m - M) * sc);
+            l += f * __hip_atomic_load(&a.part_ml[(base + z) * BR + r].y, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+            const float *p = a.part + ((base + z) * BR + r) * HD + d;
+#pragma unroll
+            for (int j = 0; j < 4; j++) o[j] += f * __hip_atomic_load(p + j, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+        }
+        store_out<HD>(a, pos0, kv, r0 + r, d, o, l);
+    }
+}
+
+// ---- shapes of a launch ------------------------------------------------------
+// Rows of a unit: 8 (PACK) or 16 while they hold all the rows of a key head,
+// else 32.
+struct Shape { int br; int64_t units; int nsplit; };
+static Shape shape_of(const EhipCache &c, int n_heads, int n_tok, int64_t tiles) {
+    Shape s;
+    const int64_t rows = (int64_t)n_tok * (n_heads / c.n_kv);
+    s.br = c.type != EHIP_KV_F32 && rows <= 8 ? 8 : rows <= 16 ? 16 : 32;
+    s.units = (rows + s.br - 1) / s.br * c.n_kv;
+    // workgroups for every CU twice, each wave at least a tile
+    const int64_t want = s.units >= 512 ? 1 : (512 + s.units - 1) / s.units, most = (tiles + AT_WAVES - 1) / AT_WAVES;
+    s.nsplit = (int)(want < most ? want : most);
+    if (s.nsplit < 1) s.nsplit = 1;
+    return s;
+}
+
+// Workspace: the units' counters (units that split are fewer than 512), then
+// the partial rows and their (maximum, sum).
+constexpr int COUNT_BYTES = 2048;
+static uint64_t space_bytes(int64_t rows, int hd) { return rows ? COUNT_BYTES + (uint64_t)rows * (4 * hd + 16) : 0; }
+static int64_t space_rows(const Shape &s) { return s.nsplit > 1 ? s.units * s.nsplit * s.br : 0; }
+
+template <int TYPE, int HD>
+static int attend_go(hipStream_t st, const AttendArgs &a, const Shape &s) {
+    const dim3 grid((unsigned)(s.units * s.nsplit)), wg(64 * AT_WAVES);
+    if constexpr (TYPE != EHIP_KV_F32) {
+        if (s.br == 8) hipLaunchKernelGGL((k_attend<TYPE, HD, 1, true>), grid, wg, 0, st, a);
+    }
+    if (s.br == 16) hipLaunchKernelGGL((k_attend<TYPE, HD, 1, false>), grid, wg, 0, st, a);
+    else if (s.br == 32) hipLaunchKernelGGL((k_attend<TYPE, HD, 2, false>), grid, wg, 0, st, a);
+    const hipError_t e = hipGetLastError();
+    return e == hipSuccess ? 0 : refuse("ehip_attend: launch: %s", hipGetErrorString(e));
+}
+
+// How a call is shared over workgroups; -1 where its workspace does not do.
+static int shape_call(const EhipCache &c, const EhipAttend &q, Shape *s) {
+    // a host position says how many tiles there are to share
+    int64_t tiles = (c.ctx + KV_TILE - 1) / KV_TILE;
+    if (!q.pos) tiles = ((int64_t)q.pos0 + q.n_tok + KV_TILE - 1) / KV_TILE;
+    if (q.window > 0) {
+        const int64_t in = ((int64_t)q.window + q.n_tok + 2 * KV_TILE) / KV_TILE + ((int64_t)q.sinks + KV_TILE - 1) / KV_TILE;
+        if (in < tiles) tiles = in;
+    }
+    *s = shape_of(c, q.n_heads, q.n_tok, tiles);
+    const uint64_t need = space_bytes(space_rows(*s), c.head_dim);
+    if (need && (!q.workspace || !aligned(q.workspace, 16) || q.workspace_bytes < need))
+        return refuse("ehip_attend: the workspace is null, not 16-byte aligned, or smaller than this call's %llu bytes", (unsigned long long)need);
+    return 0;
+}
+
+int launch_attend(hipStream_t st, const EhipCache &c, const EhipAttend &q) {
+    Shape s;
+    if (shape_call(c, q, &s)) return -1;
+    AttendArgs a{};
+    a.q = q.q; a.out = q.out; a.q_stride = q.q_stride; a.out_stride = q.out_stride;
+    a.kc = static_cast<const uint8_t *>(c.k); a.vc = static_cast<const uint8_t *>(c.v);
+    a.head_bytes = (c.ctx + KV_TILE - 1) / KV_TILE * kv_tile_bytes(c.head_dim);
+    a.kvd = c.n_kv * c.head_dim;
+    a.n_tok = q.n_tok; a.n_kv = c.n_kv; a.G = q.n_heads / c.n_kv; a.pos0 = q.pos0; a.ctx = (int)c.ctx; a.pos = q.pos;
+    a.window = q.window; a.sinks = q.sinks;
+    a.qscale = (q.scale != 0.0f ? q.scale : 1.0f / sqrtf((float)c.head_dim)) * 1.4426950408889634f;
+    a.nsplit = s.nsplit;
+    a.out_vec = aligned(q.out, 16) && q.out_stride % 4 == 0;
+    if (s.nsplit > 1) {
+        a.count = static_cast<int *>(q.workspace);
+        a.part = reinterpret_cast<float *>(static_cast<uint8_t *>(q.workspace) + COUNT_BYTES);
+        a.part_ml = reinterpret_cast<float4 *>(a.part + space_rows(s) * c.head_dim);
+    }
+    switch (c.type * 1000 + c.head_dim) {
+        case EHIP_KV_F32 * 1000 + 48: return attend_go<EHIP_KV_F32, 48>(st, a, s);
+        case EHIP_KV_F32 * 1000 + 64: return attend_go<EHIP_KV_F32, 64>(st, a, s);
+        case EHIP_KV_F32 * 1000 + 128: return attend_go<EHIP_KV_F32, 128>(st, a, s);
+        case EHIP_KV_F16 * 1000 + 48: return attend_go<EHIP_KV_F16, 48>(st, a, s);
+        case EHIP_KV_F16 * 1000 + 64: return attend_go<EHIP_KV_F16, 64>(st, a, s);
+        case EHIP_KV_F16 * 1000 + 128: return attend_go<EHIP_KV_F16, 128>(st, a, s);
+        case EHIP_KV_Q4 * 1000 + 64: return attend_go<EHIP_KV_Q4, 64>(st, a, s);
+        case EHIP_KV_Q4 * 1000 + 128: return attend_go<EHIP_KV_Q4, 128>(st, a, s);
+    }
+    return refuse("ehip_attend: head_dim %d", c.head_dim);
+}
+
+}  // namespace ehip
+
+using namespace ehip;
+
+static int check_heads(const char *who, const EhipCache *c, int n_heads, int n_tok) {
+    if (n_heads < 1 || n_heads > 65535 || n_heads % c->n_kv) return refuse("%s: %d query heads over %d key heads", who, n_heads, c->n_kv);
+    if (n_tok < 0 || n_tok > c->ctx || (int64_t)n_tok * (n_heads / c->n_kv) > INT32_MAX / 2)
+        return refuse("%s: %d tokens over a cache of %lld", who, n_tok, (long long)c->ctx);
+    return 0;
+}
+
+extern "C" uint64_t ehip_attend_workspace(const EhipCache *c, int n_heads, int n_tok) {
+    const char *who = "ehip_attend_workspace";
+    if (check_cache(who, c, false) || check_heads(who, c, n_heads, n_tok)) return 0;
+    const int G = n_heads / c->n_kv;
+    const int64_t tiles = (c->ctx + KV_TILE - 1) / KV_TILE;
+    uint64_t most = 0;
+    // the rows of a unit go through at most three sizes on the way to n_tok
+    for (int64_t rows : { (int64_t)G, (int64_t)8 / G * G, (int64_t)16 / G * G, (int64_t)n_tok * G }) {
+        if (rows < G || rows > (int64_t)n_tok * G) continue;
+        const Shape s = shape_of(*c, n_heads, (int)(rows / G), tiles);
+        // fewer units split more: 511 + units workgroups at most, however the tiles are shared
+        const int64_t units = s.units < 511 ? s.units : 511, by_tiles = units * ((tiles + AT_WAVES - 1) / AT_WAVES);
+        const int64_t wgs = 511 + units < by_tiles ? 511 + units : by_tiles;
+        const uint64_t b = wgs > units || s.nsplit > 1 ? space_bytes(wgs * s.br, c->head_dim) : 0;
+        if (b > most) most = b;
+    }
+    return most;
+}
+
+extern "C" int ehip_attend(const EhipCache *c, const EhipAttend *q, void *stream) {
+    const char *who = "ehip_attend";
+    if (!q) return refuse("%s: null argument", who);
+    if (check_cache(who, c, true) || check_heads(who, c, q->n_heads, q->n_tok)) return -1;
+    if (!q->n_tok) return 0;
+    const int64_t width = (int64_t)q->n_heads * c->head_dim;
+    if (q->n_tok > 1 && (q->q_stride < width || q->out_stride < width))
+        return refuse("%s: strides %lld and %lld for rows of %lld floats", who, (long long)q->q_stride, (long long)q->out_stride, (long long)width);
+    if (q->window < 0 || q->sinks < 0) return refuse("%s: a window of %d and %d sinks", who, q->window, q->sinks);
+    if (!(q->scale - q->scale == 0.0f)) return refuse("%s: scale %g", who, (double)q->scale);
+    if (!q->pos && (q->pos0 < 0 || (int64_t)q->pos0 + q->n_tok > c->ctx))
+        return refuse("%s: positions %d..%lld exceed the cache of %lld", who, q->pos0, (long long)q->pos0 + q->n_tok - 1, (long long)c->ctx);
+    Shape s;
+    if (shape_call(*c, *q, &s)) return -1;
+    if (!q->q || !q->out) return refuse("%s: null rows", who);
+    return launch_attend(static_cast<hipStream_t>(stream), *c, *q);
+}

@@ -129,6 +129,133 @@ int ehip_sample_noalloc(float *logits, int n, const EmberSampler *params, uint64
  * state).  Returns 0 or nonzero. */
 int ehip_noalloc_setup(void);
 
+/* ---- rotary positions, key/value caches and attention on device rows ----
+ * The parts of a layer that a long session changes, on buffers that the
+ * caller holds: positions scaled beyond the context of training, a cache in
+ * 4 bits, attention whose window ends the growth of a step.  No counterpart
+ * in the reference, whose positions, caches (src/model.c:39-80) and attention
+ * (src/model.c:207-278) are the states' above; ehip_state_create_options
+ * gives a state these instead.
+ *
+ * Pointers named x, out, q, k, v, pos, q_norm, k_norm and workspace are memory
+ * of the current device; all rows are fp32.  A call checks its description,
+ * enqueues its launches on `stream` (a hipStream_t of the current device; NULL
+ * for the default stream), allocates nothing and returns without waiting, so
+ * it can be captured into a graph.  The descriptions are read during the call
+ * only.  Zero tokens are nothing to do.  Where `pos` is given, the positions
+ * are read on the device when the launch runs (a captured step that advances),
+ * and tokens whose position lies outside the cache are left out: they store
+ * nothing and get rows of zeros.  Each returns 0, or nonzero with
+ * ehip_last_error() set. */
+
+/* How pair i's angle per position, f_i = theta^(-2i/rotary_dim), is scaled. */
+enum {
+    EHIP_ROPE_PLAIN  = 0,
+    EHIP_ROPE_LINEAR = 1, /* f / factor                                            */
+    EHIP_ROPE_NTK    = 2, /* theta * factor^(rotary_dim / (rotary_dim - 2))        */
+    EHIP_ROPE_YARN   = 3, /* f below the pair that turns `high` times in orig_ctx
+                             positions, f / factor above the one that turns `low`
+                             times, a ramp over the pair's index between them       */
+    EHIP_ROPE_BANDS  = 4  /* the same by the turns themselves: a pair of t turns gets
+                             f / factor + (f - f / factor) * clamp((t - low) / (high - low)) */
+};
+typedef struct {
+    int32_t style;        /* EMBER_ROPE_*                                           */
+    int32_t rotary_dim;   /* leading dims of each head that turn (even; 0: all)      */
+    int32_t scaling;      /* EHIP_ROPE_*                                            */
+    int32_t orig_ctx;     /* YARN, BANDS: positions of training                      */
+    float   theta, factor;
+    float   low, high;    /* YARN (both 0: 1, 32), BANDS (both 0: 1, 4)              */
+    float   magnitude;    /* cos and sin times this; 0: 0.1 ln factor + 1 for YARN with
+                             a factor above 1, else 1                                */
+} EhipRopeConfig;
+/* A configuration made ready for heads of head_dim dims: plain data of the
+ * caller's, filled by ehip_rope_plan (a host function; no GPU is needed). */
+typedef struct {
+    int32_t  style, head_dim, rotary_dim;
+    float    magnitude;
+    uint64_t turns[128];  /* pair i's angle per position, in 2^-64 of a full turn    */
+} EhipRopePlan;
+int ehip_rope_plan(const EhipRopeConfig *cfg, int head_dim, EhipRopePlan *plan);
+/* Rows of n_q query heads followed by n_k key heads, turned to their
+ * positions: each head is first normalized (RMSNorm with q_norm / k_norm,
+ * head_dim weights; NULL: not), then its leading rotary_dim dims rotate.
+ * out may be x.  head_dim is even and at most 256; any position is good. */
+typedef struct {
+    const float   *x;
+    float         *out;
+    int64_t        x_stride, out_stride;  /* floats between tokens                   */
+    int32_t        n_tok, n_q, n_k;
+    int32_t        pos0;                  /* token i's position is pos0 + i ...       */
+    const int32_t *pos;                   /* ... or pos[i] (device), where not NULL   */
+    const float   *q_norm, *k_norm;
+    float          eps;
+} EhipRopeRows;
+int ehip_rope_rows(const EhipRopePlan *plan, const EhipRopeRows *rows, void *stream);
+
+/* A layer's cache.  EHIP_KV_F32 and EHIP_KV_F16: rows [ctx][n_kv * head_dim],
+ * as the states hold them.  EHIP_KV_Q4: Q4_0 blocks of 32 dims (an fp16 scale
+ * and 32 codes, by ember_quant_q4_row's arithmetic; a block whose scale would
+ * not be a finite fp16 number reads back as NaN), for head_dim 64 and 128, in
+ * tiles of 32 positions [n_kv][(ctx + 31) / 32][18 * head_dim bytes].  A tile
+ * holds 16 * head_dim bytes of codes, then its scales:
+ *   codes   dwords at [piece][lane g * 16 + l][4], dword e of a lane in piece
+ *           e / 4 (e < head_dim / 16), nibble n at bit 4 n:
+ *           keys    e = s * head_dim / 32 + b: position 16 s + l, dim 32 b + 8 g + n
+ *           values  dim 16 e + l, position 16 (n / 4) + 4 g + n % 4
+ *   scales  fp16 at [g][b][i][s]: position 16 s + 4 g + i, block b
+ * (s, l, b, g: position half, lane, block, lane quarter; i < 4, s < 2, g < 4) */
+enum { EHIP_KV_F32 = 0, EHIP_KV_F16 = 1, EHIP_KV_Q4 = 2 };
+typedef struct {
+    void   *k, *v;       /* device, 16-byte aligned, ehip_cache_bytes each           */
+    int64_t ctx;         /* positions it holds (at most 2^30)                        */
+    int32_t type;        /* EHIP_KV_*                                               */
+    int32_t n_kv, head_dim;
+    int32_t reserved;    /* 0                                                        */
+} EhipCache;
+/* Bytes of the keys (and of the values); 0 for a shape that is not supported:
+ * head_dim 48, 64 or 128 (EHIP_KV_Q4: 64 or 128). */
+uint64_t ehip_cache_bytes(const EhipCache *cache);
+/* n_tok rows of keys and values (n_kv * head_dim floats each) into positions
+ * pos0 .. or *pos .. (device).  Calls that may run at the same time must not
+ * store into the same 32 positions (positions 32 j .. 32 j + 31). */
+typedef struct {
+    const float   *k, *v;
+    int64_t        k_stride, v_stride;    /* floats between tokens                   */
+    int32_t        n_tok, pos0;
+    const int32_t *pos;                   /* the first token's position, or NULL     */
+} EhipCacheRows;
+int ehip_cache_store(const EhipCache *cache, const EhipCacheRows *rows, void *stream);
+/* n_pos rows from position pos0 on as fp32: which = 0 keys, 1 values. */
+int ehip_cache_load(const EhipCache *cache, int which, int64_t pos0, int n_pos, float *out, int64_t out_stride, void *stream);
+
+/* Attention of n_tok tokens at positions pos0 .. (or *pos ..), whose keys and
+ * values are in the cache, over it: token at position p sees the positions
+ * t <= p, with a window > 0 only those with t > p - window or t < sinks.
+ * Query head h of a token uses key head h / (n_heads / n_kv).  out rows:
+ * softmax(q.k * scale) v.  What a token does not see does not reach its rows,
+ * whatever the cache holds there; a row that sees keys or values that are not
+ * finite need not be finite. */
+typedef struct {
+    const float   *q;
+    float         *out;
+    int64_t        q_stride, out_stride;  /* floats between tokens                   */
+    int32_t        n_tok, n_heads, pos0;
+    int32_t        window, sinks;         /* window 0: none (sinks then say nothing)  */
+    float          scale;                 /* 0: 1 / sqrt(head_dim)                   */
+    const int32_t *pos;                   /* the first token's position, or NULL     */
+    void          *workspace;             /* ehip_attend_workspace bytes, 16-byte aligned,
+                                             its first 2048 zero before its first call;
+                                             calls that may run at the same time need
+                                             one each                                 */
+    uint64_t       workspace_bytes;
+} EhipAttend;
+/* Bytes that ehip_attend needs for up to n_tok tokens of n_heads heads over
+ * this cache (its pointers are not read); 0 also where none are needed or the
+ * shape is not supported. */
+uint64_t ehip_attend_workspace(const EhipCache *cache, int n_heads, int n_tok);
+int ehip_attend(const EhipCache *cache, const EhipAttend *call, void *stream);
+
 /* One tensor for the requantizer: `rows` x `cols` fp32 values (row-major,
  * host memory, cols a multiple of 32) to be encoded as `dtype`
  * (EMBER_DT_Q8_0: 34-byte blocks, EMBER_DT_Q4_0: 18-byte blocks) into
