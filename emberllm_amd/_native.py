@@ -135,6 +135,12 @@ class EhipAttend(ctypes.Structure):
                 ("workspace_bytes", ctypes.c_uint64)]
 
 
+class EhipStateOptions(ctypes.Structure):
+    """ehip.h EhipStateOptions: a state's cache type, window, sinks and scaling."""
+    _fields_ = [("kv_type", ctypes.c_int32), ("window", ctypes.c_int32), ("sinks", ctypes.c_int32),
+                ("rope", ctypes.POINTER(EhipRopeConfig))]
+
+
 assert ctypes.sizeof(EhipRopeConfig) == 36 and ctypes.sizeof(EhipRopePlan) == 1040
 assert ctypes.sizeof(EhipRopeRows) == 80 and ctypes.sizeof(EhipCache) == 40
 assert ctypes.sizeof(EhipCacheRows) == 48 and ctypes.sizeof(EhipAttend) == 80
@@ -209,6 +215,8 @@ PROTOTYPES = {
     "ehip_cache_load": (ctypes.c_int, [ctypes.POINTER(EhipCache), ctypes.c_int, ctypes.c_int64, ctypes.c_int, _P,
                                        ctypes.c_int64, _P]),
     "ehip_attend_workspace": (ctypes.c_uint64, [ctypes.POINTER(EhipCache), ctypes.c_int, ctypes.c_int]),
+    "ehip_state_create_options": (_P, [_P, ctypes.c_int, ctypes.POINTER(EhipStateOptions)]),
+    "ember_state_new_options": (_P, [_P, ctypes.c_int, ctypes.POINTER(EhipStateOptions)]),
     "ehip_attend": (ctypes.c_int, [ctypes.POINTER(EhipCache), ctypes.POINTER(EhipAttend), _P]),
     # ember_synth.h
     "ember_synth_write": (ctypes.c_int, [ctypes.c_char_p, ctypes.POINTER(EmberSynthConfig)]),

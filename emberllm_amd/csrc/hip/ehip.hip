@@ -24,8 +24,10 @@
 
 #include "../../../include/ember.h"
 #include "../../../include/ehip.h"
+#include "../host/model_internal.h"
 #include "kernels.h"
 #include "libm_expf.h"
+#include "session.h"
 #include "staging.h"
 
 using namespace ehip;
@@ -476,6 +478,15 @@ struct EhipState {
     StepGraph smp[2];   // device sampling loop: 1 step, GEN_UNROLL steps
     SampleParams smp_graph_p; int smp_graph_cap;
     hipEvent_t ev0, ev1;
+    // a state with options (ehip_state_create_options): rotation, cache and
+    // attention of a layer by the device-row operators, on this plan, these
+    // caches (kc and vc, layer after layer) and this workspace
+    bool opt = false;
+    int window = 0, sinks = 0, kv_type = EHIP_KV_F32;
+    EhipRopePlan plan{};
+    size_t layer_bytes = 0;   // of a layer's keys, and of its values
+    void *at_ws = nullptr;
+    uint64_t at_ws_bytes = 0;
     // per-layer capture of the decode step's intermediate vectors
     // (ehip_debug_capture): layer, or -1; one device buffer per DBG_* slot
     int dbg_layer = -1;
@@ -555,7 +566,7 @@ static int env_int(const char *name, int dflt) {
 static int xm_probe(EhipState *s) {
     const int nkv = s->m->cfg.n_kv_heads, gx = 8 * s->xm_slots;
     s->xm_on = false;
-    if (!env_int("EHIP_XMERGE", 1) || s->ref_order) return 0;
+    if (!env_int("EHIP_XMERGE", 1) || s->ref_order || s->opt) return 0;
     std::vector<int> h((size_t)gx, -1);
     int *d = nullptr;
     HCHK(hipMalloc(&d, 4 * h.size()), -1);
@@ -606,7 +617,45 @@ static int xm_fallback(EhipState *s) {
     return 0;
 }
 
-extern "C" EhipState *ehip_state_create(EhipModel *m, int ctx, int kv_fp16) {
+static EhipCache layer_cache(const EhipState *s, int l) {
+    const EhipConfig &c = s->m->cfg;
+    EhipCache k{};
+    k.k = static_cast<uint8_t *>(s->kc) + (size_t)l * s->layer_bytes;
+    k.v = static_cast<uint8_t *>(s->vc) + (size_t)l * s->layer_bytes;
+    k.ctx = s->ctx; k.type = s->kv_type; k.n_kv = c.n_kv_heads; k.head_dim = c.head_dim;
+    return k;
+}
+
+// The checks and the plan of a state's options; -1 with ehip_last_error() set.
+static int take_options(EhipState *s, const EhipStateOptions *o) {
+    const char *who = "ehip_state_create_options";
+    const EhipConfig &c = s->m->cfg;
+    if (s->ref_order) return refuse("%s: EHIP_ORDER=reference has no options", who);
+    if (o->window < 0 || o->sinks < 0) return refuse("%s: a window of %d and %d sinks", who, o->window, o->sinks);
+    s->opt = true;
+    s->window = o->window; s->sinks = o->sinks; s->kv_type = o->kv_type;
+    s->f16kv = o->kv_type == EHIP_KV_F16; s->esize = s->f16kv ? 2 : 4;
+    EhipRopeConfig r{};
+    r.style = c.rope_style; r.theta = c.rope_theta;
+    if (ehip_rope_plan(o->rope ? o->rope : &r, c.head_dim, &s->plan)) return -1;
+    const EhipCache k = layer_cache(s, 0);
+    if (check_cache(who, &k, false)) return -1;
+    s->layer_bytes = (ehip_cache_bytes(&k) + 255) & ~(size_t)255;
+    s->at_ws_bytes = std::max(ehip_attend_workspace(&k, c.n_heads, 1), ehip_attend_workspace(&k, c.n_heads, std::min(PF_CHUNK, s->ctx)));
+    return 0;
+}
+
+static EhipState *create_state(EhipModel *m, int ctx, int kv_fp16, const EhipStateOptions *options);
+
+extern "C" EhipState *ehip_state_create(EhipModel *m, int ctx, int kv_fp16) { return create_state(m, ctx, kv_fp16, nullptr); }
+
+extern "C" EhipState *ehip_state_create_options(EhipModel *m, int ctx, const EhipStateOptions *options) {
+    if (!m || !options) { set_err("ehip_state_create_options: null argument"); return nullptr; }
+    if (ctx < 1) { set_err("ehip_state_create_options: a context of %d", ctx); return nullptr; }
+    return create_state(m, ctx, 0, options);
+}
+
+static EhipState *create_state(EhipModel *m, int ctx, int kv_fp16, const EhipStateOptions *options) {
     const EhipConfig &c = m->cfg;
     const int hd = c.head_dim, qd = c.n_heads * hd, kvd = c.n_kv_heads * hd;
     EhipState *s = new EhipState();  // value-initialised: every pointer starts null
@@ -615,12 +664,20 @@ extern "C" EhipState *ehip_state_create(EhipModel *m, int ctx, int kv_fp16) {
     s->graph_test_fail = env_int("EHIP_GRAPH_TEST_FAIL", 0);
     s->fw_spin = env_int("EHIP_FW_TEST_SPIN", ATT_DEC_FW_SPIN);
     s->tok_skew = env_int("EHIP_XMERGE_TEST_TOK", 0);
+    {
+        const char *ord = getenv("EHIP_ORDER");
+        s->ref_order = ord && !strcmp(ord, "reference");
+    }
+    if (options && take_options(s, options)) {
+        delete s;
+        return nullptr;
+    }
     if (hipStreamCreateWithFlags(&s->st, hipStreamNonBlocking) != hipSuccess) {
         set_err("hipStreamCreate failed");
         delete s;
         return nullptr;
     }
-    const size_t kvb = (size_t)c.n_layers * ctx * kvd * s->esize;
+    const size_t kvb = (size_t)c.n_layers * (s->opt ? s->layer_bytes : (size_t)ctx * kvd * s->esize);
     int n_cu = 0;
     if (hipDeviceGetAttribute(&n_cu, hipDeviceAttributeMultiprocessorCount, 0) != hipSuccess || n_cu <= 0) n_cu = 1;
     s->mc_dec = attn_decode_chunks(ctx, c.n_kv_heads, hd, n_cu);
@@ -645,10 +702,6 @@ extern "C" EhipState *ehip_state_create(EhipModel *m, int ctx, int kv_fp16) {
     const size_t ex_ldk = s->pf_mode == PF_EXACT ? ldk_max : (size_t)attn_prefill_ldk(0, std::min(PF_EXACT_KEYS, ctx));
     const int wide = std::max(std::max(c.dim, c.hidden_dim), qd);
     s->pf_seq = wide < GEMM_SPLIT_MIN_K;
-    {
-        const char *ord = getenv("EHIP_ORDER");
-        s->ref_order = ord && !strcmp(ord, "reference");
-    }
     bool ok = (s->kc = salloc(s, kvb, true)) && (s->vc = salloc(s, kvb, true)) &&
               (s->tokpos_d = (int *)salloc(s, 16, true)) &&
               (s->x = (float *)salloc(s, 4 * (size_t)c.dim)) &&
@@ -688,16 +741,17 @@ extern "C" EhipState *ehip_state_create(EhipModel *m, int ctx, int kv_fp16) {
               (s->wo_flag = (int *)salloc(s, 4 * (size_t)c.n_layers * c.n_kv_heads * XM_CNT_STRIDE, true));
     if (ok && m->any_f32) ok = (s->xf = (float *)salloc(s, 4 * pfc * wide)) != nullptr;
     if (ok && s->ref_order) ok = (s->att_ref = (float *)salloc(s, 4 * (size_t)c.n_heads * ctx)) != nullptr;
-    if (ok && s->pf_mode != PF_EXACT && attn_kvimg_bytes(hd, s->f16kv, ctx, c.n_kv_heads) > 0) {
+    if (ok && s->at_ws_bytes) ok = (s->at_ws = salloc(s, s->at_ws_bytes, true)) != nullptr;
+    if (ok && !s->opt && s->pf_mode != PF_EXACT && attn_kvimg_bytes(hd, s->f16kv, ctx, c.n_kv_heads) > 0) {
         s->pf_kvimg_tiles = (ctx + 63) / 64;
         ok = (s->pf_kvimg = (uint8_t *)salloc(s, attn_kvimg_bytes(hd, s->f16kv, ctx, c.n_kv_heads))) != nullptr;
     }
-    if (ok && s->pf_mode != PF_MFMA)
+    if (ok && !s->opt && s->pf_mode != PF_MFMA)
         ok = (s->pf_scores = (float *)salloc(s, 4 * ex_rows * ex_ldk * c.n_heads)) &&
              (s->pf_rowinv = (float *)salloc(s, 4 * ex_rows * c.n_heads)) &&
              (s->pf_rowmax = (float *)salloc(s, 4 * ex_rows * c.n_heads)) &&
              (s->pf_tmax = (float *)salloc(s, 4 * ex_rows * c.n_heads * (size_t)attn_prefill_tiles((int)ex_ldk)));
-    if (ok) {
+    if (ok && !s->opt) {
         // RoPE table with the reference's arithmetic (model.c:69-71): the
         // angle pos * freq in fp32, then the host libm cosf / sinf
         const int half = hd / 2;
@@ -736,6 +790,17 @@ extern "C" EhipState *ehip_state_create(EhipModel *m, int ctx, int kv_fp16) {
     memset(s->tokpos_h, 0, 16);
     *s->done_h = 0;
     return s;
+}
+
+extern "C" EmberState *ember_state_new_options(const EmberModel *mc, int ctx_len, const EhipStateOptions *o) {
+    if (!mc) { set_err("ember_state_new_options: null model"); return nullptr; }
+    EmberModel *m = const_cast<EmberModel *>(mc);   // (the device weights are its cache)
+    // scaled positions reach as far beyond the context of training
+    double most = m->hdr->max_seq_len;
+    if (o && o->rope && o->rope->scaling != EHIP_ROPE_PLAIN && o->rope->factor > 1.0f) most *= o->rope->factor;
+    const int limit = (int)std::min(most, 1073741824.0);
+    const int ctx = ctx_len <= 0 ? m->hdr->max_seq_len : std::min(ctx_len, limit);
+    return ember_state_around(m, ctx, ehip_state_create_options(ember_model_on_device(m), ctx, o));
 }
 
 // ------------------------------------------------------------ schedules ----
@@ -791,7 +856,30 @@ static bool fw_usable(EhipState *s) {
     return true;
 }
 
+// A layer's rotation (QK-norm before it), cache store and attention on n raw
+// q|k|v rows of a state with options, at pos0 .. or from the device's position.
+static int enq_session_attn(EhipState *s, int l, float *qkv, int n, int pos0, const int *pos, float *out) {
+    const EhipConfig &c = s->m->cfg;
+    const DevLayer &y = s->m->layers[l];
+    const int qd = c.n_heads * c.head_dim, kvd = c.n_kv_heads * c.head_dim, stride = qd + 2 * kvd;
+    EhipRopeRows r{};
+    r.x = qkv; r.out = qkv; r.x_stride = r.out_stride = stride;
+    r.n_tok = n; r.n_q = c.n_heads; r.n_k = c.n_kv_heads; r.pos0 = pos0; r.pos = pos;
+    r.q_norm = y.q_norm; r.k_norm = y.k_norm; r.eps = c.norm_eps;
+    if (launch_rope(s->st, s->plan, r)) return -1;
+    const EhipCache k = layer_cache(s, l);
+    EhipCacheRows w{};
+    w.k = qkv + qd; w.v = qkv + qd + kvd; w.k_stride = w.v_stride = stride; w.n_tok = n; w.pos0 = pos0; w.pos = pos;
+    if (launch_cache_store(s->st, k, w)) return -1;
+    EhipAttend a{};
+    a.q = qkv; a.out = out; a.q_stride = stride; a.out_stride = qd;
+    a.n_tok = n; a.n_heads = c.n_heads; a.pos0 = pos0; a.pos = pos; a.window = s->window; a.sinks = s->sinks;
+    a.workspace = s->at_ws; a.workspace_bytes = s->at_ws_bytes;
+    return launch_attend(s->st, k, a);
+}
+
 static int enq_attn_decode(EhipState *s, int l, bool with_merge = true, bool fw = false) {
+    if (s->opt) return enq_session_attn(s, l, s->qkv, 1, 0, s->tokpos_d + 1, s->o);
     AttnArgs a = attn_args(s, l);
     a.q = s->qkv; a.q_stride = 0; a.tokpos = s->tokpos_d; a.pos_base = 0; a.n_tok = 1;
     if (s->ref_order) {
@@ -1274,15 +1362,15 @@ static int enq_prefill_pass(EhipState *s, int pos0, int mt, bool last, int pass)
             // head per workgroup leaves most CUs without weights to fetch
             // (Qwen3-0.6B shape, 2 tokens 1059 -> 938 us, 16 tokens 1197 ->
             // 1107, 32 tokens 1193 -> 1217; 64-dim heads: no gain)
-            const bool raw = !exact && attn_raw_rows(hd, c.n_heads / c.n_kv_heads, mt) && (few ? hd == 128 && mt <= 16 : any_f32);
+            const bool raw = !s->opt && !exact && attn_raw_rows(hd, c.n_heads / c.n_kv_heads, mt) && (few ? hd == 128 && mt <= 16 : any_f32);
             bool img_fused = false;   // the q|k|v product wrote the pass's K/V tile images
             // the matrix-core attention's K/V tile images of the pass, in the
             // fused q|k|v epilogues (EHIP_PF_KVIMG=0 leaves them to
             // k_pf_kvsplit)
-            const bool img_ok = !exact && (hd == 64 || hd == 128) && s->pf_kvimg && pos0 % 64 == 0 &&
+            const bool img_ok = !s->opt && !exact && (hd == 64 || hd == 128) && s->pf_kvimg && pos0 % 64 == 0 &&
                                 s->pf_kvimg_tiles >= (pos0 + mt + 63) / 64 &&
                                 !attn_few_rows(hd, c.n_heads / c.n_kv_heads, pos0, mt) && env_int("EHIP_PF_KVIMG", 1);
-            if (raw) {
+            if (raw || s->opt) {
                 rc |= few ? launch_few_store(s->st, g, NormIn{s->X, y.attn_norm, c.norm_eps}) : launch_gemm(s->st, EPI_STORE, g);
                 if (psnap(DBG_QKV, s->QKV, stride, stride)) return -1;
             } else if (few) {
@@ -1331,7 +1419,8 @@ static int enq_prefill_pass(EhipState *s, int pos0, int mt, bool last, int pass)
             // weights, whose product reads the fp32 rows)
             bool quantized = false;
             if (!any_f32) { at.qx = s->qx; at.qdx = s->dxp; at.qxs = s->xsum; }
-            rc |= exact ? launch_attention(s->st, s->f16kv, at, &quantized)
+            rc |= s->opt ? enq_session_attn(s, l, s->QKV, mt, pos0, nullptr, s->O)
+                : exact ? launch_attention(s->st, s->f16kv, at, &quantized)
                 : raw ? launch_attention_raw(s->st, s->f16kv, at, &quantized)
                       : launch_attention_mfma(s->st, s->f16kv, at, &quantized);
             if (psnap(DBG_O, s->O, qd, qd)) return -1;
@@ -1453,24 +1542,54 @@ extern "C" float *ehip_prefill(EhipState *s, const int *ids, int n, int start) {
 
 
 // ------------------------------------------------------- inspection ----
-extern "C" int ehip_kv_read(EhipState *s, int which, int layer, int n_pos, void *host) {
+// A 4-bit layer's rows as the format's blocks ([n_pos][n_kv * hd / 32] of 18
+// bytes) from or into its tiles, both in host memory.
+static void q4_rows(const EhipConfig &c, uint8_t *tiles, int ntiles, bool values, int n_pos, uint8_t *rows, bool write) {
+    const int hd = c.head_dim, nb = hd / QB;
+    for (int p = 0; p < n_pos; p++)
+        for (int kv = 0; kv < c.n_kv_heads; kv++)
+            for (int b = 0; b < nb; b++) {
+                uint8_t *blk = rows + (((size_t)p * c.n_kv_heads + kv) * nb + b) * 18;
+                uint8_t *tile = tiles + ((size_t)kv * ntiles + p / KV_TILE) * kv_tile_bytes(hd);
+                const int s = p % KV_TILE / 16, g = p % 16 / 4, i = p % 4;
+                uint8_t *scale = tile + kv_scale_at(hd, g, b, i, s);
+                if (write) memcpy(scale, blk, 2);
+                else memcpy(blk, scale, 2);
+                for (int j = 0; j < QB; j++) {
+                    const int nib = values ? 4 * s + i : j % 8;
+                    uint8_t *code = tile + nib / 2 + (values ? kv_code_at(g * 16 + j % 16, 2 * b + j / 16) : kv_code_at(j / 8 * 16 + p % 16, s * nb + b));
+                    uint8_t *to = blk + 2 + j % 16;
+                    const int up = 4 * (nib & 1), rup = j < 16 ? 0 : 4;
+                    if (write) *code = (uint8_t)((*code & ~(15 << up)) | ((*to >> rup & 15) << up));
+                    else *to = (uint8_t)((*to & ~(15 << rup)) | ((*code >> up & 15) << rup));
+                }
+            }
+}
+
+static int kv_copy(EhipState *s, int which, int layer, int n_pos, void *host, bool write) {
     const EhipConfig &c = s->m->cfg;
-    const size_t row = (size_t)c.n_kv_heads * c.head_dim * s->esize;
-    if (layer < 0 || layer >= c.n_layers || n_pos < 0 || n_pos > s->ctx) { set_err("kv_read out of range"); return -1; }
-    const uint8_t *base = static_cast<const uint8_t *>(which ? s->vc : s->kc) + (size_t)layer * s->ctx * row;
+    if (layer < 0 || layer >= c.n_layers || n_pos < 0 || n_pos > s->ctx) { set_err("kv_%s out of range", write ? "write" : "read"); return -1; }
     HCHK(hipStreamSynchronize(s->st), -1);
-    HCHK(hipMemcpy(host, base, row * n_pos, hipMemcpyDeviceToHost), -1);
+    const size_t row = (size_t)c.n_kv_heads * c.head_dim * s->esize, layer_bytes = s->opt ? s->layer_bytes : (size_t)s->ctx * row;
+    uint8_t *base = static_cast<uint8_t *>(which ? s->vc : s->kc) + (size_t)layer * layer_bytes;
+    if (s->opt && s->kv_type == EHIP_KV_Q4) {
+        std::vector<uint8_t> tiles(layer_bytes);
+        HCHK(hipMemcpy(tiles.data(), base, layer_bytes, hipMemcpyDeviceToHost), -1);
+        q4_rows(c, tiles.data(), (s->ctx + KV_TILE - 1) / KV_TILE, which != 0, n_pos, static_cast<uint8_t *>(host), write);
+        if (write) HCHK(hipMemcpy(base, tiles.data(), layer_bytes, hipMemcpyHostToDevice), -1);
+        return 0;
+    }
+    if (write) HCHK(hipMemcpy(base, host, row * n_pos, hipMemcpyHostToDevice), -1);
+    else HCHK(hipMemcpy(host, base, row * n_pos, hipMemcpyDeviceToHost), -1);
     return 0;
 }
 
+extern "C" int ehip_kv_read(EhipState *s, int which, int layer, int n_pos, void *host) {
+    return kv_copy(s, which, layer, n_pos, host, false);
+}
+
 extern "C" int ehip_kv_write(EhipState *s, int which, int layer, int n_pos, const void *host) {
-    const EhipConfig &c = s->m->cfg;
-    const size_t row = (size_t)c.n_kv_heads * c.head_dim * s->esize;
-    if (layer < 0 || layer >= c.n_layers || n_pos < 0 || n_pos > s->ctx) { set_err("kv_write out of range"); return -1; }
-    uint8_t *base = static_cast<uint8_t *>(which ? s->vc : s->kc) + (size_t)layer * s->ctx * row;
-    HCHK(hipStreamSynchronize(s->st), -1);
-    HCHK(hipMemcpy(base, host, row * n_pos, hipMemcpyHostToDevice), -1);
-    return 0;
+    return kv_copy(s, which, layer, n_pos, const_cast<void *>(host), true);
 }
 
 extern "C" int ehip_debug_buffer(EhipState *s, int which, void *host, uint64_t bytes) {

@@ -118,19 +118,31 @@ EmberState *ember_state_new(const EmberModel *m, int ctx_len) {
     return ember_state_new_ex(m, ctx_len, 0);
 }
 
+EhipModel *ember_model_on_device(EmberModel *m) {
+    if (!m->dev) upload(m);
+    return m->dev;
+}
+
+EmberState *ember_state_around(EmberModel *m, int ctx, EhipState *dev) {
+    if (!dev) return NULL;
+    EmberState *s = ember_xcalloc(1, sizeof *s, "EmberState");
+    s->m = m;
+    s->ctx = ctx;
+    s->vocab = m->hdr->vocab_size;
+    s->dev = dev;
+    s->zeros = ember_xcalloc((size_t)s->vocab, sizeof(float), "logits");
+    s->logits = s->zeros;
+    return s;
+}
+
 EmberState *ember_state_new_ex(const EmberModel *mc, int ctx_len, int kv_fp16) {
     EmberModel *m = (EmberModel *)mc;  /* the device weight cache is mutable state of the model */
     const EmberHeader *h = m->hdr;
-    if (!m->dev) upload(m);
-    EmberState *s = ember_xcalloc(1, sizeof *s, "EmberState");
-    s->m = m;
-    s->ctx = (ctx_len > 0 && ctx_len < h->max_seq_len) ? ctx_len : h->max_seq_len;
-    s->vocab = h->vocab_size;
-    if (s->ctx <= 0) ember_die("model has no usable context length");
-    s->dev = ehip_state_create(m->dev, s->ctx, kv_fp16 ? 1 : 0);
-    if (!s->dev) ember_die("device state creation failed: %s", ehip_last_error());
-    s->zeros = ember_xcalloc((size_t)s->vocab, sizeof(float), "logits");
-    s->logits = s->zeros;
+    EhipModel *dm = ember_model_on_device(m);
+    const int ctx = (ctx_len > 0 && ctx_len < h->max_seq_len) ? ctx_len : h->max_seq_len;
+    if (ctx <= 0) ember_die("model has no usable context length");
+    EmberState *s = ember_state_around(m, ctx, ehip_state_create(dm, ctx, kv_fp16 ? 1 : 0));
+    if (!s) ember_die("device state creation failed: %s", ehip_last_error());
     return s;
 }
 

@@ -20,4 +20,15 @@ struct EmberModel {
 /* Free the device copy of the weights (called by ember_model_free). */
 void ember_model_release_device(EmberModel *m);
 
+#ifdef __cplusplus
+extern "C" {
+#endif
+/* The model's weights on the GPU, uploaded by the first call. */
+EhipModel *ember_model_on_device(EmberModel *m);
+/* The state around a device state of `ctx` positions; NULL for NULL. */
+EmberState *ember_state_around(EmberModel *m, int ctx, EhipState *dev);
+#ifdef __cplusplus
+}
+#endif
+
 #endif

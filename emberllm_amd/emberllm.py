@@ -13,19 +13,38 @@ from . import _native
 
 
 class Engine:
-    """A loaded model and one device state, with numpy results."""
+    """A loaded model and one device state, with numpy results.
 
-    def __init__(self, path, ctx=0, kv_fp16=False):
+    kv ("f32", "f16" or "q4"), window, sinks or rope (an
+    _native.EhipRopeConfig) make a state with options
+    (ember_state_new_options): its cache's type, a sliding window with first
+    positions that stay visible, scaled positions."""
+
+    def __init__(self, path, ctx=0, kv_fp16=False, kv=None, window=0, sinks=0, rope=None):
         self.lib = _native.lib()
         self.m = self.lib.ember_model_load(path.encode())
         if not self.m:
             raise RuntimeError(f"failed to load model: {path}")
         self.header = self.lib.ember_model_header(self.m).contents
-        self.st = self.lib.ember_state_new_ex(self.m, int(ctx), 1 if kv_fp16 else 0)
         maxs = self.header.max_seq_len
-        self.ctx = maxs if ctx <= 0 or ctx > maxs else ctx
+        self.kv = kv or ("f16" if kv_fp16 else "f32")
+        if kv is None and not window and not sinks and rope is None:
+            self.st = self.lib.ember_state_new_ex(self.m, int(ctx), 1 if kv_fp16 else 0)
+        else:
+            types = {"f32": _native.KV_F32, "f16": _native.KV_F16, "q4": _native.KV_Q4}
+            if self.kv not in types:
+                raise ValueError(f"unknown cache type {kv!r}")
+            opt = _native.EhipStateOptions(kv_type=types[self.kv], window=int(window), sinks=int(sinks))
+            if rope is not None:
+                opt.rope = ctypes.pointer(rope)
+                if rope.scaling != _native.ROPE_PLAIN and rope.factor > 1:
+                    maxs = int(min(maxs * rope.factor, 1 << 30))
+            self.st = self.lib.ember_state_new_options(self.m, int(ctx), ctypes.byref(opt))
+            if not self.st:
+                raise RuntimeError(_native.last_error())
+        self.ctx = self.header.max_seq_len if ctx <= 0 else min(int(ctx), maxs)
         self.vocab = self.header.vocab_size
-        self.kv_fp16 = bool(kv_fp16)
+        self.kv_fp16 = self.kv == "f16"
         self.dev = self.lib.ember_state_device(self.st)
 
     def forward(self, tok, pos):
@@ -40,7 +59,8 @@ class Engine:
 
     def kv_row_bytes(self):
         h = self.header
-        return h.n_kv_heads * h.head_dim * (2 if self.kv_fp16 else 4)
+        n = h.n_kv_heads * h.head_dim
+        return n // 32 * 18 if self.kv == "q4" else n * (2 if self.kv_fp16 else 4)
 
     def kv_read(self, which, layer, n_pos):
         out = np.empty(n_pos * self.kv_row_bytes(), dtype=np.uint8)

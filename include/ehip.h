@@ -256,6 +256,23 @@ typedef struct {
 uint64_t ehip_attend_workspace(const EhipCache *cache, int n_heads, int n_tok);
 int ehip_attend(const EhipCache *cache, const EhipAttend *call, void *stream);
 
+/* A state whose layers rotate, cache and attend by the operators above: its
+ * decode steps, prefill passes and device loops are those of any state, with
+ * up to `ctx` positions.  ehip_kv_read / ehip_kv_write give an EHIP_KV_Q4 cache
+ * as rows of the format's 18-byte blocks; ehip_time_kernel's kernel 0 is the
+ * rotation, the store and the attention of a layer. */
+typedef struct {
+    int32_t kv_type;             /* EHIP_KV_*                                       */
+    int32_t window, sinks;       /* as in EhipAttend                                */
+    const EhipRopeConfig *rope;  /* NULL: the model's style and theta, unscaled     */
+} EhipStateOptions;
+EhipState *ehip_state_create_options(EhipModel *m, int ctx, const EhipStateOptions *options);
+/* The same beneath an EmberState for ember_forward, ember_prefill and
+ * ember_state_free.  ctx_len as in ember_state_new, except that a rope factor
+ * above 1 allows for up to max_seq_len * factor positions.  NULL with
+ * ehip_last_error() set for options that are refused. */
+EmberState *ember_state_new_options(const EmberModel *m, int ctx_len, const EhipStateOptions *options);
+
 /* One tensor for the requantizer: `rows` x `cols` fp32 values (row-major,
  * host memory, cols a multiple of 32) to be encoded as `dtype`
  * (EMBER_DT_Q8_0: 34-byte blocks, EMBER_DT_Q4_0: 18-byte blocks) into
