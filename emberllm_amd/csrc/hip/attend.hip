@@ -62,6 +62,7 @@ struct AttendArgs {
     int *count;                  // [unit]: workgroups of the unit that are done; zero between launches
 };
 
+constexpr int AT_SPLITS = 64;    // workgroups that a unit's tiles are shared over at most
 constexpr int AT_WAVES = 4;      // waves of a workgroup: they share its rows and take tiles in turn
 
 // maximum / sum over the four lane quarters of a row
@@ -700,44 +701,61 @@ __global__ __launch_bounds__(64 * AT_WAVES) void k_attend(AttendArgs a) {
         if (alone) {
             store_out<HD>(a, pos0, kv, r0 + r, d, o, l);
         } else {
-            // agent scope: another XCD's workgroup reads them
-            float *p = a.part + (slot * BR + r) * HD + d;
-#pragma unroll
-            for (int j = 0; j < 4; j++) __hip_atomic_store(p + j, o[j], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-            if (d == 0) {
-                __hip_atomic_store(&a.part_ml[slot * BR + r].x, M, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-                __hip_atomic_store(&a.part_ml[slot * BR + r].y, l, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-                __hip_atomic_store(&a.part_ml[slot * BR + r].z, ssc[r], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-            }
+            *reinterpret_cast<f32x4 *>(a.part + (slot * BR + r) * HD + d) = o;
+            if (d == 0) a.part_ml[slot * BR + r] = make_float4(M, l, ssc[r], 0.0f);
         }
     }
     if (alone) return;
 
-    // ---- the unit's workgroups: the last one to arrive joins the runs
-    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "agent");
+    // ---- the unit's workgroups: the last one to arrive joins the runs.  Every
+    // wave's stores have completed before the release (which writes this L2
+    // back for the other XCDs); the acquire makes theirs visible here.
+    __builtin_amdgcn_s_waitcnt(0);
     __syncthreads();
-    if (tid == 0) s_last = __hip_atomic_fetch_add(a.count + unit, 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == nact - 1;
+    if (tid == 0) s_last = __hip_atomic_fetch_add(a.count + unit, 1, __ATOMIC_ACQ_REL, __HIP_MEMORY_SCOPE_AGENT) == nact - 1;
     __syncthreads();
     if (!s_last) return;
-    __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "agent");
     if (tid == 0) __hip_atomic_store(a.count + unit, 0, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
     const int64_t base = (int64_t)unit * a.nsplit;
-    for (int i = tid; i < (r1 - r0) * (HD / 4); i += 64 * AT_WAVES) {
-        const int r = i / (HD / 4), d = i % (HD / 4) * 4;
-        const float sc = __hip_atomic_load(&a.part_ml[base * BR + r].z, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-        float M = -INFINITY;
-        for (int z = 0; z < nact; z++) M = fmaxf(M, __hip_atomic_load(&a.part_ml[(base + z) * BR + r].x, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT));
+    float *sf = &so[0][0][0];                       // [row][AT_SPLITS]: the runs' weights over the row's sum
+    f32x4 *red = reinterpret_cast<f32x4 *>(sf + BR * AT_SPLITS);
+    static_assert(BR * AT_SPLITS * 4 + 64 * AT_WAVES * 16 <= sizeof(so), "the join fits the waves' outputs");
+    const int nr = r1 - r0;
+    for (int r = wave; r < nr; r += AT_WAVES) {     // a wave a row, a lane a run: one round trip
+        const float4 ml = a.part_ml[(base + min(lane, nact - 1)) * BR + r];
+        const float m = lane < nact ? ml.x : -INFINITY, M = wave_max(m);
+        const float f = m == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f((m - M) * ml.z);
+        const float l = wave_sum(lane < nact ? f * ml.y : 0.0f);
+        sf[r * AT_SPLITS + lane] = f;
+        if (lane == 0) sl[0][r] = l;
+    }
+    __syncthreads();
+    // an item is four dims of a row; with fewer items than threads they share the runs
+    const int items = nr * (HD / 4), parts = max(64 * AT_WAVES / items, 1);
+    for (int i0 = 0; i0 < items; i0 += 64 * AT_WAVES) {
+        const int part = parts > 1 ? tid / items : 0, i = parts > 1 ? tid % items : i0 + tid;
+        const int r = min(i, items - 1) / (HD / 4), d = i % (HD / 4) * 4;
         f32x4 o = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
-        float l = 0.0f;
-        for (int z = 0; z < nact; z++) {
-            const float m = __hip_atomic_load(&a.part_ml[(base + z) * BR + r].x, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-            const float f = m == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f((m - M) * sc);
-            l += f * __hip_atomic_load(&a.part_ml[(base + z) * BR + r].y, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-            const float *p = a.part + ((base + z) * BR + r) * HD + d;
+        if (i < items && part < parts) {
+            const float *p = a.part + (base * BR + r) * HD + d;
+            for (int z = part; z < nact; z += 8 * parts) {
+                f32x4 x[8];
 #pragma unroll
-            for (int j = 0; j < 4; j++) o[j] += f * __hip_atomic_load(p + j, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+                for (int j = 0; j < 8; j++) x[j] = *reinterpret_cast<const f32x4 *>(p + (int64_t)min(z + j * parts, nact - 1) * (BR * HD));
+#pragma unroll
+                for (int j = 0; j < 8; j++) {
+                    const float f = z + j * parts < nact ? sf[r * AT_SPLITS + z + j * parts] : 0.0f;
+                    o += x[j] * f;
+                }
+            }
         }
-        store_out<HD>(a, pos0, kv, r0 + r, d, o, l);
+        if (parts > 1) {
+            red[tid] = o;
+            __syncthreads();
+            if (tid >= items) return;
+            for (int q = 1; q < parts; q++) o += red[q * items + tid];
+        }
+        if (i < items) store_out<HD>(a, pos0, kv, r0 + r, d, o, sl[0][r]);
     }
 }
 
@@ -753,6 +771,7 @@ static Shape shape_of(const EhipCache &c, int n_heads, int n_tok, int64_t tiles)
     // workgroups for every CU twice, each wave at least a tile
     const int64_t want = s.units >= 512 ? 1 : (512 + s.units - 1) / s.units, most = (tiles + AT_WAVES - 1) / AT_WAVES;
     s.nsplit = (int)(want < most ? want : most);
+    if (s.nsplit > AT_SPLITS) s.nsplit = AT_SPLITS;
     if (s.nsplit < 1) s.nsplit = 1;
     return s;
 }
