@@ -24,24 +24,25 @@
 // products and sums are fp32.  q is scaled per row (its largest element into
 // [2^13, 2^14)), times scale * log2(e) first, so the scores are in log2 units.
 // Codes are exact in fp16; a score is the sum over its blocks of (block's
-// product) * d in fp32.  For P.V each block's scale goes into the
-// probability: w_t d_t, times 2^E with E from the largest |d| so far, keeps
-// both halves in fp16's range (below 2^15: what a half loses at its smallest
-// is 2^-38 of the largest).  The outputs' sums carry 2^E until the end.  An
-// fp16 cache is exact already and has E = 14; an fp32 cache goes through the
-// fp32 matrix cores as it is, with E = 0.
+// product) * d in fp32.  A value (code - 8) d has at most 15 bits, so hi =
+// fp16((code - 8) d) and lo = (code - 8) d - hi hold it exactly at any fp16 d.
+// Probabilities are split times 2^14 (what a half loses at its smallest is
+// 2^-39 of the largest), which the outputs' sums carry until the end; of the
+// four products of halves the smallest, lo.lo below 2^-24 of the whole, is
+// left out where it is not free.  fp16 caches are one half already; an fp32
+// cache goes through the fp32 matrix cores as it is.
 //
 // What a row does not see cannot reach it: its scores are selected away, its
 // probabilities are zero, and where a zero times what the cache holds would be
-// NaN (infinite or NaN values, scales of positions never stored) the factor is
-// selected away too (4 bits: the scale) or the value's products are made one
-// by one for the rows that see it.
+// NaN (infinite or NaN values, scales of positions never stored) a 4-bit scale
+// becomes zero and the scores of the rows that see it NaN, and an fp16 or fp32
+// value's products are made one by one for the rows that see it.
 #include "session.h"
 
 namespace ehip {
 
 typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
-typedef unsigned short u16x2 __attribute__((ext_vector_type(2)));
+typedef float f32x2 __attribute__((ext_vector_type(2)));
 typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
 
 struct AttendArgs {
@@ -78,8 +79,12 @@ __device__ __forceinline__ uint32_t pack2(_Float16 a, _Float16 b) {
     return (uint32_t)__builtin_bit_cast(uint16_t, a) | ((uint32_t)__builtin_bit_cast(uint16_t, b) << 16);
 }
 __device__ __forceinline__ f16x8 as_f16(i32x4 v) { return __builtin_bit_cast(f16x8, v); }
-// fp16 number in half s of a dword, widened
-__device__ __forceinline__ float half_of(int w, int s) { return (float)__builtin_bit_cast(f16x2, w)[s]; }
+// a dword's two fp16 numbers, and back (by value: __builtin_bit_cast of a
+// vector's element takes its first one)
+__device__ __forceinline__ f16x2 halves(int w) { return __builtin_bit_cast(f16x2, w); }
+__device__ __forceinline__ int dword(f16x2 h) { return __builtin_bit_cast(int, h); }
+// number s, widened
+__device__ __forceinline__ float half_of(int w, int s) { return (float)halves(w)[s]; }
 
 // The 8 codes of a dword, minus 8, as fp16 pairs (n, n + 4), n = 0 .. 3; the
 // pairs of odd n come 16 times too large, which their partner operand makes
@@ -87,7 +92,7 @@ __device__ __forceinline__ float half_of(int w, int s) { return (float)__builtin
 // nibble) or 16 times it.
 __device__ __forceinline__ i32x4 codes_signed(uint32_t w) {
     const f16x2 lo = { (_Float16)-1032.0f, (_Float16)-1032.0f }, hi = { (_Float16)-1152.0f, (_Float16)-1152.0f };
-    auto one = [](uint32_t bits, f16x2 off) { return __builtin_bit_cast(int, __builtin_bit_cast(f16x2, bits) + off); };
+    auto one = [](uint32_t bits, f16x2 off) { return dword(halves((int)bits) + off); };
     const uint32_t v = w >> 8;
     return i32x4{ one((w & 0x000f000fu) | 0x64006400u, lo), one((w & 0x00f000f0u) | 0x64006400u, hi),
                   one((v & 0x000f000fu) | 0x64006400u, lo), one((v & 0x00f000f0u) | 0x64006400u, hi) };
@@ -230,20 +235,22 @@ __device__ __forceinline__ f32x4 add_halves(f32x4 v) {
     return v;
 }
 
-// The hi and lo halves of 8 probabilities w[s][i] as the P operand: pairs
-// (s = 0, s = 1) of i.
+// The hi and lo halves of 8 probabilities, times even / odd by i, as the P
+// operand: pairs (s = 0, s = 1) of i.
 template <bool PACK>
-__device__ __forceinline__ void split_p(const float (&w)[2][4], i32x4 &hi, i32x4 &lo) {
+__device__ __forceinline__ void split_p(const f32x4 (&p)[2], float even, float odd, i32x4 &hi, i32x4 &lo) {
     const bool low = PACK && ((threadIdx.x & 8) != 0);
 #pragma unroll
     for (int i = 0; i < 4; i++) {
-        const _Float16 a = (_Float16)w[0][i], b = (_Float16)w[1][i];
-        const _Float16 la = (_Float16)(w[0][i] - (float)a), lb = (_Float16)(w[1][i] - (float)b);
+        const f32x2 w = f32x2{ p[0][i] * (i & 1 ? odd : even), p[1][i] * (i & 1 ? odd : even) };
+        const f16x2 h = __builtin_convertvector(w, f16x2);
+        const f32x2 rest = f32x2{ w[0] - (float)h[0], w[1] - (float)h[1] };
         if (PACK) {
-            hi[i] = (int)(low ? pack2(la, lb) : pack2(a, b));
+            const f32x2 mine = f32x2{ low ? rest[0] : w[0], low ? rest[1] : w[1] };
+            hi[i] = dword(__builtin_convertvector(mine, f16x2));
         } else {
-            hi[i] = (int)pack2(a, b);
-            lo[i] = (int)pack2(la, lb);
+            hi[i] = dword(h);
+            lo[i] = dword(__builtin_convertvector(rest, f16x2));
         }
     }
 }
@@ -256,8 +263,7 @@ template <int HD, int CT, bool PACK> struct Tile<EHIP_KV_Q4, HD, CT, PACK> {
     static constexpr int NB = HD / QB, NP = HD / 64;
     i32x4 k[NP], v[NP], ks[NB], vs[NB];
     QHalf<HD, CT, PACK> Q;
-    int top = 0x0400;            // the largest |d| of a value so far (fp16 bits), at least 2^-14
-    int E = 29 - (0x0400 >> 10);   // |d| < 2^((top >> 10) - 14): the factors stay below 2^15
+    int E = 14;                  // the outputs' sums carry 2^E: 14, or 6 once a value was 4096 and more
     const uint8_t *kb, *vb;
 
     __device__ __forceinline__ void init(const AttendArgs &a, int kv) {
@@ -306,76 +312,74 @@ template <int HD, int CT, bool PACK> struct Tile<EHIP_KV_Q4, HD, CT, PACK> {
             if (PACK) S[0][s] = add_halves(S[0][s]);
         }
     }
-    // masked: t0 the tile's first position, lo_seen / hi_seen the positions that any row sees
-    template <bool MASKED>
-    __device__ __forceinline__ void values(const AttendArgs &a, Rows<HD, CT> &R, f32x4 (&S)[CT][2], int t0, int kv, int first_pos, int last_pos) {
-        const int g = (threadIdx.x & 63) >> 4;
-        // the largest finite |d| among the positions that a row sees
-        u16x2 mx = { 0, 0 };
+    // whether a value's 16 times too large codes can leave fp16: |d| of 512 and more (not NaN)
+    __device__ __forceinline__ bool large() const {
+        int any = 0;
 #pragma unroll
         for (int b = 0; b < NB; b++)
 #pragma unroll
-            for (int i = 0; i < 4; i++) {
-                u16x2 w = __builtin_bit_cast(u16x2, vs[b][i] & 0x7fff7fff);
-                if (MASKED) {
+            for (int i = 0; i < 4; i++) any |= vs[b][i];
+        if (!__any((any & 0x6000) == 0x6000 || (any & 0x60000000) == 0x60000000)) return false;   // (no |d| has both exponent bits)
+        bool big = false;
 #pragma unroll
-                    for (int s = 0; s < 2; s++) {
-                        const int t = t0 + 16 * s + 4 * g + i;
-                        if (!(t <= last_pos && (a.window <= 0 || t > first_pos - a.window || t < a.sinks))) w[s] = 0;
-                    }
+        for (int b = 0; b < NB; b++)
+#pragma unroll
+            for (int i = 0; i < 4; i++)
+#pragma unroll
+                for (int s = 0; s < 2; s++) {
+                    const int d = vs[b][i] >> (16 * s) & 0x7fff;
+                    big |= d >= 0x6000 && d < 0x7c00;
                 }
-                mx = __builtin_elementwise_max(mx, w);
-            }
-        int big = max((int)mx[0], (int)mx[1]);
-        if (__any(big >= 0x7c00)) {   // the block of a NaN: its rows' sums are NaN at any E
-            big = 0;
-#pragma unroll
-            for (int b = 0; b < NB; b++)
-#pragma unroll
-                for (int i = 0; i < 4; i++)
-#pragma unroll
-                    for (int s = 0; s < 2; s++) {
-                        const int t = t0 + 16 * s + 4 * g + i, w = vs[b][i] >> (16 * s) & 0x7fff;
-                        if (w < 0x7c00 && t <= last_pos && (a.window <= 0 || t > first_pos - a.window || t < a.sinks)) big = max(big, w);
-                    }
-        }
-        big = max(big, __shfl_xor(big, 16));
-        big = max(big, __shfl_xor(big, 32));
-        top = max(top, big);
-        const int En = 29 - (top >> 10);
-        softmax_step(R, S, __builtin_amdgcn_ldexpf(1.0f, En - E));
-        E = En;
-        const float even = __builtin_amdgcn_ldexpf(1.0f, E), odd = even * 0.0625f;   // (the codes of odd i are 16 times too large)
-#pragma unroll
-        for (int c = 0; c < CT; c++)
+        return __any(big);
+    }
+    template <bool MASKED>
+    __device__ __forceinline__ void values(const AttendArgs &, Rows<HD, CT> &R, f32x4 (&S)[CT][2], int, int, int) {
+        if (MASKED) {   // scales that are not finite: their rows' scores are not, and the values zero
 #pragma unroll
             for (int s = 0; s < 2; s++)
 #pragma unroll
-                for (int i = 0; i < 4; i++) S[c][s][i] *= i & 1 ? odd : even;
+                for (int i = 0; i < 4; i++) {
+                    const int expo = 0x7c00 << (16 * s);
+                    bool bad = false;
 #pragma unroll
-        for (int b = 0; b < NB; b++) {
-            const i32x4 c0 = codes_signed((uint32_t)v[(2 * b) >> 2][(2 * b) & 3]), c1 = codes_signed((uint32_t)v[(2 * b + 1) >> 2][(2 * b + 1) & 3]);
+                    for (int b = 0; b < NB; b++) bad |= (vs[b][i] & expo) == expo;
+#pragma unroll
+                    for (int b = 0; b < NB; b++) vs[b][i] = bad ? vs[b][i] & (s ? 0xffff : (int)0xffff0000) : vs[b][i];
+#pragma unroll
+                    for (int c = 0; c < CT; c++) S[c][s][i] = bad && S[c][s][i] != -INFINITY ? __builtin_nanf("") : S[c][s][i];
+                }
+        }
+        const bool big = large();
+        softmax_step(R, S, big && E == 14 ? 0x1p-8f : 1.0f);
+        if (big) {
+            E = 6;
+            const f16x2 down = { (_Float16)0x1p-8f, (_Float16)0x1p-8f };
+#pragma unroll
+            for (int b = 0; b < NB; b++)
+#pragma unroll
+                for (int i = 0; i < 4; i++) vs[b][i] = dword(halves(vs[b][i]) * down);
+        }
+        const float even = big || E == 14 ? 0x1p14f : 0x1p6f, odd = even * 0.0625f;   // (the codes of odd i are 16 times too large)
+        i32x4 hi[CT], lo[CT];
+#pragma unroll
+        for (int c = 0; c < CT; c++) split_p<PACK>(S[c], even, odd, hi[c], lo[c]);
+#pragma unroll
+        for (int d = 0; d < HD / 16; d++) {
+            const i32x4 code = codes_signed((uint32_t)v[d >> 2][d & 3]);
+            i32x4 vh, vl;
+#pragma unroll
+            for (int i = 0; i < 4; i++) {
+                const f16x2 x = halves(code[i]), y = halves(vs[d >> 1][i]), h = x * y;
+                vh[i] = dword(h);
+                vl[i] = dword(__builtin_elementwise_fma(x, y, -h));
+            }
 #pragma unroll
             for (int c = 0; c < CT; c++) {
-                float w[2][4];
-#pragma unroll
-                for (int s = 0; s < 2; s++)
-#pragma unroll
-                    for (int i = 0; i < 4; i++) {
-                        w[s][i] = S[c][s][i] * half_of(vs[b][i], s);
-                        if (MASKED && !seen(a, R, c, t0 + 16 * s + 4 * g + i)) w[s][i] = 0.0f;
-                    }
-                i32x4 hi, lo;
-                split_p<PACK>(w, hi, lo);
-                R.o[c][2 * b] = mfma16(c0, hi, R.o[c][2 * b]);
-                R.o[c][2 * b + 1] = mfma16(c1, hi, R.o[c][2 * b + 1]);
-                if (!PACK) {
-                    R.o[c][2 * b] = mfma16(c0, lo, R.o[c][2 * b]);
-                    R.o[c][2 * b + 1] = mfma16(c1, lo, R.o[c][2 * b + 1]);
-                }
+                R.o[c][d] = mfma16(vl, hi[c], R.o[c][d]);
+                if (!PACK) R.o[c][d] = mfma16(vh, lo[c], R.o[c][d]);
+                R.o[c][d] = mfma16(vh, hi[c], R.o[c][d]);
             }
         }
-        (void)kv;
     }
     __device__ __forceinline__ int exponent() const { return E; }
 };
@@ -465,7 +469,7 @@ template <int HD, int CT, bool PACK> struct Tile<EHIP_KV_F16, HD, CT, PACK> {
             }
     }
     template <bool MASKED>
-    __device__ __forceinline__ void values(const AttendArgs &a, Rows<HD, CT> &R, f32x4 (&S)[CT][2], int t0, int kv, int, int last_pos) {
+    __device__ __forceinline__ void values(const AttendArgs &a, Rows<HD, CT> &R, f32x4 (&S)[CT][2], int t0, int kv, int last_pos) {
         bool odd = false;
         if (MASKED) {   // what is not finite goes to its own rows only
 #pragma unroll
@@ -481,13 +485,8 @@ template <int HD, int CT, bool PACK> struct Tile<EHIP_KV_F16, HD, CT, PACK> {
         softmax_step(R, S, 1.0f);
 #pragma unroll
         for (int c = 0; c < CT; c++) {
-            float w[2][4];
-#pragma unroll
-            for (int s = 0; s < 2; s++)
-#pragma unroll
-                for (int i = 0; i < 4; i++) w[s][i] = S[c][s][i] * 16384.0f;
             i32x4 hi, lo;
-            split_p<PACK>(w, hi, lo);
+            split_p<PACK>(S[c], 0x1p14f, 0x1p14f, hi, lo);
 #pragma unroll
             for (int d = 0; d < HD / 16; d++) {
                 R.o[c][d] = mfma16(v[d], hi, R.o[c][d]);
@@ -554,7 +553,7 @@ template <int HD, int CT, bool PACK> struct Tile<EHIP_KV_F32, HD, CT, PACK> {
             }
     }
     template <bool MASKED>
-    __device__ __forceinline__ void values(const AttendArgs &a, Rows<HD, CT> &R, f32x4 (&S)[CT][2], int t0, int kv, int, int last_pos) {
+    __device__ __forceinline__ void values(const AttendArgs &a, Rows<HD, CT> &R, f32x4 (&S)[CT][2], int t0, int kv, int last_pos) {
         bool odd = false;
         if (MASKED) {
 #pragma unroll
@@ -654,10 +653,10 @@ __global__ __launch_bounds__(64 * AT_WAVES) void k_attend(AttendArgs a) {
         vi += AT_WAVES;
         if (vi < v1) X.load_k(a, T.at(vi), last_pos);
         if (whole) {
-            X.template values<false>(a, R, S, t0, kv, first_pos, last_pos);
+            X.template values<false>(a, R, S, t0, kv, last_pos);
         } else {
             mask_scores(a, R, S, t0);
-            X.template values<true>(a, R, S, t0, kv, first_pos, last_pos);
+            X.template values<true>(a, R, S, t0, kv, last_pos);
         }
         if (vi < v1) X.load_v(a, T.at(vi), last_pos);
     }
