@@ -597,6 +597,24 @@ __device__ __forceinline__ void store_out(const AttendArgs &a, int pos0, int kv,
     }
 }
 
+// 16 bytes that workgroups of other XCDs read or have written: agent scope,
+// so they pass the XCD's L2 both ways (a release and acquire per workgroup
+// instead writes back and drops a whole L2 each time: 512 workgroups 17 us
+// where 264 take 12)
+__device__ __forceinline__ void put_part(float *p, f32x4 v) {
+    typedef unsigned long long u64x2 __attribute__((ext_vector_type(2)));
+    const u64x2 w = __builtin_bit_cast(u64x2, v);
+    unsigned long long *q = reinterpret_cast<unsigned long long *>(p);
+    __hip_atomic_store(q, w[0], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    __hip_atomic_store(q + 1, w[1], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+}
+__device__ __forceinline__ f32x4 get_part(const float *p) {
+    typedef unsigned long long u64x2 __attribute__((ext_vector_type(2)));
+    const unsigned long long *q = reinterpret_cast<const unsigned long long *>(p);
+    const u64x2 w = u64x2{ __hip_atomic_load(q, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT), __hip_atomic_load(q + 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) };
+    return __builtin_bit_cast(f32x4, w);
+}
+
 // ---- the kernel ------------------------------------------------------------
 // Workgroup (unit, split): unit = (row group, key head), key heads fastest so
 // that a key head's workgroups share an XCD's L2; row groups from the last, so
@@ -700,18 +718,18 @@ __global__ __launch_bounds__(64 * AT_WAVES) void k_attend(AttendArgs a) {
         if (alone) {
             store_out<HD>(a, pos0, kv, r0 + r, d, o, l);
         } else {
-            *reinterpret_cast<f32x4 *>(a.part + (slot * BR + r) * HD + d) = o;
-            if (d == 0) a.part_ml[slot * BR + r] = make_float4(M, l, ssc[r], 0.0f);
+            put_part(a.part + (slot * BR + r) * HD + d, o);
+            if (d == 0) put_part(reinterpret_cast<float *>(a.part_ml + slot * BR + r), f32x4{M, l, ssc[r], 0.0f});
         }
     }
     if (alone) return;
 
     // ---- the unit's workgroups: the last one to arrive joins the runs.  Every
-    // wave's stores have completed before the release (which writes this L2
-    // back for the other XCDs); the acquire makes theirs visible here.
+    // wave's partial stores have completed, past its XCD's L2, before the
+    // workgroup counts itself, and the last one's loads go past its own.
     __builtin_amdgcn_s_waitcnt(0);
     __syncthreads();
-    if (tid == 0) s_last = __hip_atomic_fetch_add(a.count + unit, 1, __ATOMIC_ACQ_REL, __HIP_MEMORY_SCOPE_AGENT) == nact - 1;
+    if (tid == 0) s_last = __hip_atomic_fetch_add(a.count + unit, 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == nact - 1;
     __syncthreads();
     if (!s_last) return;
     if (tid == 0) __hip_atomic_store(a.count + unit, 0, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
@@ -721,10 +739,10 @@ __global__ __launch_bounds__(64 * AT_WAVES) void k_attend(AttendArgs a) {
     static_assert(BR * AT_SPLITS * 4 + 64 * AT_WAVES * 16 <= sizeof(so), "the join fits the waves' outputs");
     const int nr = r1 - r0;
     for (int r = wave; r < nr; r += AT_WAVES) {     // a wave a row, a lane a run: one round trip
-        const float4 ml = a.part_ml[(base + min(lane, nact - 1)) * BR + r];
-        const float m = lane < nact ? ml.x : -INFINITY, M = wave_max(m);
-        const float f = m == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f((m - M) * ml.z);
-        const float l = wave_sum(lane < nact ? f * ml.y : 0.0f);
+        const f32x4 ml = get_part(reinterpret_cast<const float *>(a.part_ml + (base + min(lane, nact - 1)) * BR + r));
+        const float m = lane < nact ? ml[0] : -INFINITY, M = wave_max(m);
+        const float f = m == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f((m - M) * ml[2]);
+        const float l = wave_sum(lane < nact ? f * ml[1] : 0.0f);
         sf[r * AT_SPLITS + lane] = f;
         if (lane == 0) sl[0][r] = l;
     }
@@ -740,7 +758,7 @@ __global__ __launch_bounds__(64 * AT_WAVES) void k_attend(AttendArgs a) {
             for (int z = part; z < nact; z += 8 * parts) {
                 f32x4 x[8];
 #pragma unroll
-                for (int j = 0; j < 8; j++) x[j] = *reinterpret_cast<const f32x4 *>(p + (int64_t)min(z + j * parts, nact - 1) * (BR * HD));
+                for (int j = 0; j < 8; j++) x[j] = get_part(p + (int64_t)min(z + j * parts, nact - 1) * (BR * HD));
 #pragma unroll
                 for (int j = 0; j < 8; j++) {
                     const float f = z + j * parts < nact ? sf[r * AT_SPLITS + z + j * parts] : 0.0f;
