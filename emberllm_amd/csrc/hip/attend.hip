@@ -64,7 +64,6 @@ struct AttendArgs {
 };
 
 constexpr int AT_SPLITS = 64;    // workgroups that a unit's tiles are shared over at most
-constexpr int AT_WAVES = 4;      // waves of a workgroup: they share its rows and take tiles in turn
 
 // maximum / sum over the four lane quarters of a row
 __device__ __forceinline__ float quarters_max(float v) {
@@ -89,13 +88,19 @@ __device__ __forceinline__ float half_of(int w, int s) { return (float)halves(w)
 // The 8 codes of a dword, minus 8, as fp16 pairs (n, n + 4), n = 0 .. 3; the
 // pairs of odd n come 16 times too large, which their partner operand makes
 // up.  0x6400 is 1024, whose last mantissa bits take a code as it lies (the low
-// nibble) or 16 times it.
-__device__ __forceinline__ i32x4 codes_signed(uint32_t w) {
+// nibble) or 16 times it.  magic: 0x64006400 in a vector register, so that a
+// mask and it make one instruction (v_and_or_b32 takes one scalar).
+__device__ __forceinline__ uint32_t code_magic() {
+    uint32_t m = 0x64006400u;
+    asm volatile("" : "+v"(m));
+    return m;
+}
+__device__ __forceinline__ i32x4 codes_signed(uint32_t w, uint32_t magic) {
     const f16x2 lo = { (_Float16)-1032.0f, (_Float16)-1032.0f }, hi = { (_Float16)-1152.0f, (_Float16)-1152.0f };
     auto one = [](uint32_t bits, f16x2 off) { return dword(halves((int)bits) + off); };
     const uint32_t v = w >> 8;
-    return i32x4{ one((w & 0x000f000fu) | 0x64006400u, lo), one((w & 0x00f000f0u) | 0x64006400u, hi),
-                  one((v & 0x000f000fu) | 0x64006400u, lo), one((v & 0x00f000f0u) | 0x64006400u, hi) };
+    return i32x4{ one((w & 0x000f000fu) | magic, lo), one((w & 0x00f000f0u) | magic, hi),
+                  one((v & 0x000f000fu) | magic, lo), one((v & 0x00f000f0u) | magic, hi) };
 }
 
 // Which tiles of 32 positions the rows r0 .. r1 - 1 of a launch see: the sinks'
@@ -265,12 +270,12 @@ template <int HD, int CT, bool PACK> struct Tile<EHIP_KV_Q4, HD, CT, PACK> {
     QHalf<HD, CT, PACK> Q;
     int E = 14;                  // the outputs' sums carry 2^E: 14, or 6 once a value was 4096 and more
     const uint8_t *kb, *vb;
+    uint32_t magic;
 
     __device__ __forceinline__ void init(const AttendArgs &a, int kv) {
-        const int lane = threadIdx.x & 63;
+        magic = code_magic();
         kb = a.kc + kv * a.head_bytes;
         vb = a.vc + kv * a.head_bytes;
-        (void)lane;
     }
     __device__ __forceinline__ void load_q(const AttendArgs &a, const float *row, int c, float &sc) {
         load_q16<HD, CT, PACK, true>(a, row, c, Q, sc);
@@ -299,7 +304,7 @@ template <int HD, int CT, bool PACK> struct Tile<EHIP_KV_Q4, HD, CT, PACK> {
 #pragma unroll
             for (int b = 0; b < NB; b++) {
                 const int e = s * NB + b;
-                const i32x4 codes = codes_signed((uint32_t)k[e >> 2][e & 3]);
+                const i32x4 codes = codes_signed((uint32_t)k[e >> 2][e & 3], magic);
 #pragma unroll
                 for (int c = 0; c < CT; c++) {
                     f32x4 x = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
@@ -324,12 +329,15 @@ template <int HD, int CT, bool PACK> struct Tile<EHIP_KV_Q4, HD, CT, PACK> {
 #pragma unroll
         for (int b = 0; b < NB; b++)
 #pragma unroll
-            for (int i = 0; i < 4; i++)
+            for (int i = 0; i < 4; i++) {
+                int w = vs[b][i];
+                asm volatile("" : "+v"(w));   // (stays in this branch: the exact test is rare)
 #pragma unroll
                 for (int s = 0; s < 2; s++) {
-                    const int d = vs[b][i] >> (16 * s) & 0x7fff;
+                    const int d = w >> (16 * s) & 0x7fff;
                     big |= d >= 0x6000 && d < 0x7c00;
                 }
+            }
         return __any(big);
     }
     template <bool MASKED>
@@ -365,7 +373,7 @@ template <int HD, int CT, bool PACK> struct Tile<EHIP_KV_Q4, HD, CT, PACK> {
         for (int c = 0; c < CT; c++) split_p<PACK>(S[c], even, odd, hi[c], lo[c]);
 #pragma unroll
         for (int d = 0; d < HD / 16; d++) {
-            const i32x4 code = codes_signed((uint32_t)v[d >> 2][d & 3]);
+            const i32x4 code = codes_signed((uint32_t)v[d >> 2][d & 3], magic);
             i32x4 vh, vl;
 #pragma unroll
             for (int i = 0; i < 4; i++) {
@@ -619,15 +627,15 @@ __device__ __forceinline__ f32x4 get_part(const float *p) {
 // Workgroup (unit, split): unit = (row group, key head), key heads fastest so
 // that a key head's workgroups share an XCD's L2; row groups from the last, so
 // that the longest start first.  The unit's nsplit workgroups take equal runs
-// of its tiles (those without one leave), and the wave w of a workgroup the
-// tiles w, w + 4, ... of the run.  The last workgroup of a unit to arrive puts
+// of its tiles (those without one leave), and the wave w of a workgroup's NW
+// the tiles w, w + NW, ... of the run.  The last workgroup of a unit to arrive puts
 // the runs together.
-template <int TYPE, int HD, int CT, bool PACK>
-__global__ __launch_bounds__(64 * AT_WAVES) void k_attend(AttendArgs a) {
+template <int TYPE, int HD, int CT, bool PACK, int NW>
+__global__ __launch_bounds__(64 * NW) void k_attend(AttendArgs a) {
     constexpr int BR = PACK ? 8 : 16 * CT;        // rows of a unit
     constexpr int LD = HD + 4;                    // floats between rows in LDS
-    __shared__ __align__(16) float so[AT_WAVES][BR][LD];
-    __shared__ float sm[AT_WAVES][BR], sl[AT_WAVES][BR], ssc[BR], se[AT_WAVES];
+    __shared__ __align__(16) float so[NW][BR][LD];
+    __shared__ float sm[NW][BR], sl[NW][BR], ssc[BR], se[NW];
     __shared__ int s_last;
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, g = lane >> 4;
     const int nunits = gridDim.x / a.nsplit;
@@ -668,7 +676,7 @@ __global__ __launch_bounds__(64 * AT_WAVES) void k_attend(AttendArgs a) {
         const bool whole = t0 + KV_TILE - 1 <= all_to && (t0 >= all_from || t0 + KV_TILE <= a.sinks);
         f32x4 S[CT][2];
         X.scores(S);
-        vi += AT_WAVES;
+        vi += NW;
         if (vi < v1) X.load_k(a, T.at(vi), last_pos);
         if (whole) {
             X.template values<false>(a, R, S, t0, kv, last_pos);
@@ -701,15 +709,15 @@ __global__ __launch_bounds__(64 * AT_WAVES) void k_attend(AttendArgs a) {
     __syncthreads();
     const bool alone = nact == 1;
     const int64_t slot = (int64_t)unit * a.nsplit + split;
-    for (int i = tid; i < BR * (HD / 4); i += 64 * AT_WAVES) {
+    for (int i = tid; i < BR * (HD / 4); i += 64 * NW) {
         const int r = i / (HD / 4), d = i % (HD / 4) * 4;
         float M = sm[0][r];
 #pragma unroll
-        for (int w = 1; w < AT_WAVES; w++) M = fmaxf(M, sm[w][r]);
+        for (int w = 1; w < NW; w++) M = fmaxf(M, sm[w][r]);
         f32x4 o = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
         float l = 0.0f;
 #pragma unroll
-        for (int w = 0; w < AT_WAVES; w++) {
+        for (int w = 0; w < NW; w++) {
             const float f = sm[w][r] == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f((sm[w][r] - M) * ssc[r]);
             o += *reinterpret_cast<const f32x4 *>(&so[w][r][d]) * (f * se[w]);
             l += sl[w][r] * f;
@@ -736,9 +744,9 @@ __global__ __launch_bounds__(64 * AT_WAVES) void k_attend(AttendArgs a) {
     const int64_t base = (int64_t)unit * a.nsplit;
     float *sf = &so[0][0][0];                       // [row][AT_SPLITS]: the runs' weights over the row's sum
     f32x4 *red = reinterpret_cast<f32x4 *>(sf + BR * AT_SPLITS);
-    static_assert(BR * AT_SPLITS * 4 + 64 * AT_WAVES * 16 <= sizeof(so), "the join fits the waves' outputs");
+    static_assert(BR * AT_SPLITS * 4 + 64 * NW * 16 <= sizeof(so), "the join fits the waves' outputs");
     const int nr = r1 - r0;
-    for (int r = wave; r < nr; r += AT_WAVES) {     // a wave a row, a lane a run: one round trip
+    for (int r = wave; r < nr; r += NW) {     // a wave a row, a lane a run: one round trip
         const f32x4 ml = get_part(reinterpret_cast<const float *>(a.part_ml + (base + min(lane, nact - 1)) * BR + r));
         const float m = lane < nact ? ml[0] : -INFINITY, M = wave_max(m);
         const float f = m == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f((m - M) * ml[2]);
@@ -748,8 +756,8 @@ __global__ __launch_bounds__(64 * AT_WAVES) void k_attend(AttendArgs a) {
     }
     __syncthreads();
     // an item is four dims of a row; with fewer items than threads they share the runs
-    const int items = nr * (HD / 4), parts = max(64 * AT_WAVES / items, 1);
-    for (int i0 = 0; i0 < items; i0 += 64 * AT_WAVES) {
+    const int items = nr * (HD / 4), parts = max(64 * NW / items, 1);
+    for (int i0 = 0; i0 < items; i0 += 64 * NW) {
         const int part = parts > 1 ? tid / items : 0, i = parts > 1 ? tid % items : i0 + tid;
         const int r = min(i, items - 1) / (HD / 4), d = i % (HD / 4) * 4;
         f32x4 o = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
@@ -778,15 +786,20 @@ __global__ __launch_bounds__(64 * AT_WAVES) void k_attend(AttendArgs a) {
 
 // ---- shapes of a launch ------------------------------------------------------
 // Rows of a unit: 8 (PACK) or 16 while they hold all the rows of a key head,
-// else 32.
-struct Shape { int br; int64_t units; int nsplit; };
+// else 32.  Waves of a workgroup: 4; for few rows of a 4-bit cache 8 where 4
+// would make more workgroups than CUs, as half the ranges are then joined
+// (16 heads of 128 over 8192 positions 15.0 -> 13.4 us; over 2048, which 4
+// waves spread over more CUs, 10.0 -> 10.9; an fp32 cache, whose products are
+// longer, 54 -> 58 over 32,768).
+struct Shape { int br, waves; int64_t units; int nsplit; };
 static Shape shape_of(const EhipCache &c, int n_heads, int n_tok, int64_t tiles) {
     Shape s;
     const int64_t rows = (int64_t)n_tok * (n_heads / c.n_kv);
     s.br = c.type != EHIP_KV_F32 && rows <= 8 ? 8 : rows <= 16 ? 16 : 32;
     s.units = (rows + s.br - 1) / s.br * c.n_kv;
-    // workgroups for every CU twice, each wave at least a tile
-    const int64_t want = s.units >= 512 ? 1 : (512 + s.units - 1) / s.units, most = (tiles + AT_WAVES - 1) / AT_WAVES;
+    s.waves = c.type == EHIP_KV_Q4 && s.br <= 16 && s.units * ((tiles + 3) / 4) > 256 ? 8 : 4;
+    // 2048 waves (two to each SIMD), each with at least a tile
+    const int64_t all = 2048 / s.waves, want = s.units >= all ? 1 : (all + s.units - 1) / s.units, most = (tiles + s.waves - 1) / s.waves;
     s.nsplit = (int)(want < most ? want : most);
     if (s.nsplit > AT_SPLITS) s.nsplit = AT_SPLITS;
     if (s.nsplit < 1) s.nsplit = 1;
@@ -801,12 +814,16 @@ static int64_t space_rows(const Shape &s) { return s.nsplit > 1 ? s.units * s.ns
 
 template <int TYPE, int HD>
 static int attend_go(hipStream_t st, const AttendArgs &a, const Shape &s) {
-    const dim3 grid((unsigned)(s.units * s.nsplit)), wg(64 * AT_WAVES);
+    const dim3 grid((unsigned)(s.units * s.nsplit)), wg(64 * s.waves);
     if constexpr (TYPE != EHIP_KV_F32) {
-        if (s.br == 8) hipLaunchKernelGGL((k_attend<TYPE, HD, 1, true>), grid, wg, 0, st, a);
+        if (s.br == 8 && s.waves == 4) hipLaunchKernelGGL((k_attend<TYPE, HD, 1, true, 4>), grid, wg, 0, st, a);
     }
-    if (s.br == 16) hipLaunchKernelGGL((k_attend<TYPE, HD, 1, false>), grid, wg, 0, st, a);
-    else if (s.br == 32) hipLaunchKernelGGL((k_attend<TYPE, HD, 2, false>), grid, wg, 0, st, a);
+    if constexpr (TYPE == EHIP_KV_Q4) {
+        if (s.br == 8 && s.waves == 8) hipLaunchKernelGGL((k_attend<TYPE, HD, 1, true, 8>), grid, wg, 0, st, a);
+        if (s.br == 16 && s.waves == 8) hipLaunchKernelGGL((k_attend<TYPE, HD, 1, false, 8>), grid, wg, 0, st, a);
+    }
+    if (s.br == 16 && s.waves == 4) hipLaunchKernelGGL((k_attend<TYPE, HD, 1, false, 4>), grid, wg, 0, st, a);
+    else if (s.br == 32) hipLaunchKernelGGL((k_attend<TYPE, HD, 2, false, 4>), grid, wg, 0, st, a);
     const hipError_t e = hipGetLastError();
     return e == hipSuccess ? 0 : refuse("ehip_attend: launch: %s", hipGetErrorString(e));
 }
@@ -875,14 +892,14 @@ extern "C" uint64_t ehip_attend_workspace(const EhipCache *c, int n_heads, int n
     const int G = n_heads / c->n_kv;
     const int64_t tiles = (c->ctx + KV_TILE - 1) / KV_TILE;
     uint64_t most = 0;
-    // the rows of a unit go through at most three sizes on the way to n_tok
-    for (int64_t rows : { (int64_t)G, (int64_t)8 / G * G, (int64_t)16 / G * G, (int64_t)n_tok * G }) {
-        if (rows < G || rows > (int64_t)n_tok * G) continue;
-        const Shape s = shape_of(*c, n_heads, (int)(rows / G), tiles);
-        // fewer units split more: 511 + units workgroups at most, however the tiles are shared
-        const int64_t units = s.units < 511 ? s.units : 511, by_tiles = units * ((tiles + AT_WAVES - 1) / AT_WAVES);
-        const int64_t wgs = 511 + units < by_tiles ? 511 + units : by_tiles;
-        const uint64_t b = wgs > units || s.nsplit > 1 ? space_bytes(wgs * s.br, c->head_dim) : 0;
+    // on the way to n_tok tokens a unit's rows go through at most three sizes:
+    // the largest counts of tokens of each, with either count of waves
+    for (int64_t n : { (int64_t)1, (int64_t)8 / G, (int64_t)16 / G, (int64_t)n_tok }) {
+        if (n < 1 || n > n_tok) continue;
+        const Shape s = shape_of(*c, n_heads, (int)n, tiles);
+        const int64_t all = 512, units = s.units < all - 1 ? s.units : all - 1, by_tiles = units * ((tiles + 3) / 4);
+        const int64_t wgs = all - 1 + units < by_tiles ? all - 1 + units : by_tiles;
+        const uint64_t b = wgs > units ? space_bytes(wgs * s.br, c->head_dim) : 0;
         if (b > most) most = b;
     }
     return most;
