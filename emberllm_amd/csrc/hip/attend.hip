@@ -37,237 +37,23 @@
 // NaN (infinite or NaN values, scales of positions never stored) a 4-bit scale
 // becomes zero and the scores of the rows that see it NaN, and an fp16 or fp32
 // value's products are made one by one for the rows that see it.
-#include "session.h"
+#include "attend.h"
 
 namespace ehip {
 
-typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
-typedef float f32x2 __attribute__((ext_vector_type(2)));
-typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
-
-struct AttendArgs {
-    const float *q;
-    float *out;
-    int64_t q_stride, out_stride;
-    const uint8_t *kc, *vc;
-    int64_t head_bytes;          // 4 bits: bytes of a key head's tiles
-    int kvd;                     // others: elements of a position
-    int n_tok, n_kv, G, pos0, ctx;
-    const int *pos;
-    int out_vec;                 // out rows take 16-byte stores
-    int window, sinks;
-    float qscale;                // scale * log2(e)
-    int nsplit;                  // workgroups that share a row group's positions
-    float *part;                 // [unit][nsplit][rows][HD], then float4 [unit][nsplit][rows]; unit = (row group, key head)
-    float4 *part_ml;             // a row's maximum, sum and score scale
-    int *count;                  // [unit]: workgroups of the unit that are done; zero between launches
-};
-
-constexpr int AT_SPLITS = 64;    // workgroups that a unit's tiles are shared over at most
-
-// maximum / sum over the four lane quarters of a row
-__device__ __forceinline__ float quarters_max(float v) {
-    const auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
-    v = fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1]));
-    const auto t = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
-    return fmaxf(__uint_as_float(t[0]), __uint_as_float(t[1]));
-}
-__device__ __forceinline__ float quarters_sum(float v) { return xor32_add(xor16_add(v)); }
-
-__device__ __forceinline__ uint32_t pack2(_Float16 a, _Float16 b) {
-    return (uint32_t)__builtin_bit_cast(uint16_t, a) | ((uint32_t)__builtin_bit_cast(uint16_t, b) << 16);
-}
-__device__ __forceinline__ f16x8 as_f16(i32x4 v) { return __builtin_bit_cast(f16x8, v); }
-// a dword's two fp16 numbers, and back (by value: __builtin_bit_cast of a
-// vector's element takes its first one)
-__device__ __forceinline__ f16x2 halves(int w) { return __builtin_bit_cast(f16x2, w); }
-__device__ __forceinline__ int dword(f16x2 h) { return __builtin_bit_cast(int, h); }
-// number s, widened
-__device__ __forceinline__ float half_of(int w, int s) { return (float)halves(w)[s]; }
-
-// The 8 codes of a dword, minus 8, as fp16 pairs (n, n + 4), n = 0 .. 3; the
-// pairs of odd n come 16 times too large, which their partner operand makes
-// up.  0x6400 is 1024, whose last mantissa bits take a code as it lies (the low
-// nibble) or 16 times it.  magic: 0x64006400 in a vector register, so that a
-// mask and it make one instruction (v_and_or_b32 takes one scalar).
-__device__ __forceinline__ uint32_t code_magic() {
-    uint32_t m = 0x64006400u;
-    asm volatile("" : "+v"(m));
-    return m;
-}
-__device__ __forceinline__ i32x4 codes_signed(uint32_t w, uint32_t magic) {
-    const f16x2 lo = { (_Float16)-1032.0f, (_Float16)-1032.0f }, hi = { (_Float16)-1152.0f, (_Float16)-1152.0f };
-    auto one = [](uint32_t bits, f16x2 off) { return dword(halves((int)bits) + off); };
-    const uint32_t v = w >> 8;
-    return i32x4{ one((w & 0x000f000fu) | magic, lo), one((w & 0x00f000f0u) | magic, hi),
-                  one((v & 0x000f000fu) | magic, lo), one((v & 0x00f000f0u) | magic, hi) };
-}
-
-// Which tiles of 32 positions the rows r0 .. r1 - 1 of a launch see: the sinks'
-// tiles [0, ns), then those from w0 on; n in all, tile of index v.
-struct Tiles {
-    int ns, w0, n;
-    __device__ __forceinline__ int at(int v) const { return v < ns ? v : v - ns + w0; }
-};
-__device__ __forceinline__ Tiles tiles_seen(int first_pos, int last_pos, int window, int sinks) {
-    Tiles t;
-    const int last = last_pos / KV_TILE;
-    t.ns = 0;
-    t.w0 = 0;
-    if (window > 0) {
-        t.ns = sinks > 0 ? min((sinks - 1) / KV_TILE, last) + 1 : 0;
-        t.w0 = max(max(first_pos - window + 1, 0) / KV_TILE, t.ns);
-    }
-    t.n = t.ns + max(last + 1 - t.w0, 0);
-    return t;
-}
-
-// The rows of a wave: CT groups of 16 (PACK: one of 8, whose columns 8 .. 15
-// hold the low halves of the same rows), their running softmax and output.
-template <int HD, int CT> struct Rows {
-    float sc[CT];                // score = product * sc
-    int p[CT];                   // the row's position
-    float m[CT], l[CT];          // maximum (in products), this lane's share of the sum
-    f32x4 o[CT][HD / 16];
-};
-
-// sum and maximum updates shared by the cache types: S[c][s][i] are products
-// (masked ones -inf), which become the probabilities 2^((S - max) sc).  up: what
-// the output's sums are multiplied by beside (a new exponent), 1 mostly.
-template <int HD, int CT>
-__device__ __forceinline__ void softmax_step(Rows<HD, CT> &R, f32x4 (&S)[CT][2], float up) {
-#pragma unroll
-    for (int c = 0; c < CT; c++) {
-        float t = fmaxf(fmaxf(S[c][0][0], S[c][0][1]), fmaxf(S[c][0][2], S[c][0][3]));
-        t = fmaxf(t, fmaxf(fmaxf(S[c][1][0], S[c][1][1]), fmaxf(S[c][1][2], S[c][1][3])));
-        const float mn = fmaxf(R.m[c], quarters_max(t));
-        if (__any(mn > R.m[c]) || up != 1.0f) {
-            const float a = R.m[c] == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f((R.m[c] - mn) * R.sc[c]);
-            R.l[c] *= a;
-#pragma unroll
-            for (int d = 0; d < HD / 16; d++) R.o[c][d] *= a * up;
-            R.m[c] = mn;
-        }
-        // (the difference first: the exponential's argument is then off by
-        // its own rounding only, at whatever size the scores are)
-        const float mu = mn == -INFINITY ? 0.0f : mn;
-        float l = 0.0f;
-#pragma unroll
-        for (int s = 0; s < 2; s++)
-#pragma unroll
-            for (int i = 0; i < 4; i++) {
-                S[c][s][i] = __builtin_amdgcn_exp2f((S[c][s][i] - mu) * R.sc[c]);
-                l += S[c][s][i];
-            }
-        R.l[c] += l;
-    }
-}
-
-// the scores of positions that a row does not see become -inf
-template <int HD, int CT>
-__device__ __forceinline__ bool seen(const AttendArgs &a, const Rows<HD, CT> &R, int c, int t) {
-    return t <= R.p[c] && (a.window <= 0 || t > R.p[c] - a.window || t < a.sinks);
-}
-template <int HD, int CT>
-__device__ __forceinline__ void mask_scores(const AttendArgs &a, const Rows<HD, CT> &R, f32x4 (&S)[CT][2], int t0) {
-    const int g = (threadIdx.x & 63) >> 4;
-#pragma unroll
-    for (int c = 0; c < CT; c++)
-#pragma unroll
-        for (int s = 0; s < 2; s++)
-#pragma unroll
-            for (int i = 0; i < 4; i++)
-                if (!seen(a, R, c, t0 + 16 * s + 4 * g + i)) S[c][s][i] = -INFINITY;
-}
-
 // ---- one tile of each cache type ------------------------------------------
-// The Q operand of the fp16 matrix cores: q[c][b][0] the high halves, [1] the
-// low ones (PACK: [0] alone, high or low by the column).
-template <int HD, int CT, bool PACK> struct QHalf {
-    static constexpr int NB = (HD + 31) / 32, NH = PACK ? 1 : 2;
-    i32x4 q[CT][NB][NH];
-};
-
-// Loads a row's dims 32 b + 8 g .. + 7, scales and splits them.  ORDER4: the
-// element order of a code dword, (0, 4), (1, 5) / 16, (2, 6), (3, 7) / 16.
-template <int HD, int CT, bool PACK, bool ORDER4>
-__device__ __forceinline__ void load_q16(const AttendArgs &a, const float *row, int c, QHalf<HD, CT, PACK> &Q, float &sc) {
-    constexpr int NB = QHalf<HD, CT, PACK>::NB;
-    const int lane = threadIdx.x & 63, g = lane >> 4;
-    float x[NB][8];
-    float top = 0.0f;
-#pragma unroll
-    for (int b = 0; b < NB; b++)
-#pragma unroll
-        for (int j = 0; j < 8; j++) {
-            const int d = 32 * b + 8 * g + j;
-            x[b][j] = HD % 32 == 0 || d < HD ? row[HD % 32 == 0 ? d : min(d, HD - 1)] * a.qscale : 0.0f;
-            top = fmaxf(top, fabsf(x[b][j]));
-        }
-    top = quarters_max(top);
-    const int e = top > 0.0f ? 14 - __builtin_amdgcn_frexp_expf(top) : 0;   // top 2^e in [2^13, 2^14)
-    sc = __builtin_amdgcn_ldexpf(1.0f, -e);
-#pragma unroll
-    for (int b = 0; b < NB; b++) {
-        _Float16 hi[8], lo[8];
-#pragma unroll
-        for (int j = 0; j < 8; j++) {
-            const float y = __builtin_amdgcn_ldexpf(x[b][j], ORDER4 && (j & 1) ? e - 4 : e);
-            hi[j] = (_Float16)y;
-            lo[j] = (_Float16)(y - (float)hi[j]);
-        }
-        i32x4 h, w;
-        if (ORDER4) {
-            h = i32x4{ (int)pack2(hi[0], hi[4]), (int)pack2(hi[1], hi[5]), (int)pack2(hi[2], hi[6]), (int)pack2(hi[3], hi[7]) };
-            w = i32x4{ (int)pack2(lo[0], lo[4]), (int)pack2(lo[1], lo[5]), (int)pack2(lo[2], lo[6]), (int)pack2(lo[3], lo[7]) };
-        } else {
-            h = i32x4{ (int)pack2(hi[0], hi[1]), (int)pack2(hi[2], hi[3]), (int)pack2(hi[4], hi[5]), (int)pack2(hi[6], hi[7]) };
-            w = i32x4{ (int)pack2(lo[0], lo[1]), (int)pack2(lo[2], lo[3]), (int)pack2(lo[4], lo[5]), (int)pack2(lo[6], lo[7]) };
-        }
-        if (PACK) Q.q[c][b][0] = (lane & 8) ? w : h;
-        else { Q.q[c][b][0] = h; Q.q[c][b][QHalf<HD, CT, PACK>::NH - 1] = w; }
-    }
-}
-
-__device__ __forceinline__ f32x4 mfma16(i32x4 a, i32x4 b, f32x4 c) {
-    return __builtin_amdgcn_mfma_f32_16x16x32_f16(as_f16(a), as_f16(b), c, 0, 0, 0);
-}
-
-// rows 0 .. 7 and their low halves in columns 8 .. 15, added in both
-__device__ __forceinline__ f32x4 add_halves(f32x4 v) {
-#pragma unroll
-    for (int i = 0; i < 4; i++) v[i] = xor8_add(v[i]);
-    return v;
-}
-
-// The hi and lo halves of 8 probabilities, times even / odd by i, as the P
-// operand: pairs (s = 0, s = 1) of i.
-template <bool PACK>
-__device__ __forceinline__ void split_p(const f32x4 (&p)[2], float even, float odd, i32x4 &hi, i32x4 &lo) {
-    const bool low = PACK && ((threadIdx.x & 8) != 0);
-#pragma unroll
-    for (int i = 0; i < 4; i++) {
-        const f32x2 w = f32x2{ p[0][i] * (i & 1 ? odd : even), p[1][i] * (i & 1 ? odd : even) };
-        const f16x2 h = __builtin_convertvector(w, f16x2);
-        const f32x2 rest = f32x2{ w[0] - (float)h[0], w[1] - (float)h[1] };
-        if (PACK) {
-            const f32x2 mine = f32x2{ low ? rest[0] : w[0], low ? rest[1] : w[1] };
-            hi[i] = dword(__builtin_convertvector(mine, f16x2));
-        } else {
-            hi[i] = dword(h);
-            lo[i] = dword(__builtin_convertvector(rest, f16x2));
-        }
-    }
-}
-
-template <int TYPE, int HD, int CT, bool PACK> struct Tile;
+// QL: the rows' Q operands lie in LDS (at ql), where the workgroup's waves share
+// them, instead of in registers
+template <int TYPE, int HD, int CT, bool PACK, bool QL> struct Tile;
 
 // 4 bits: HD / 16 dwords of codes for keys and for values per lane, and the
 // scales of the lane's 8 positions (dword b * 4 + i: positions s = 0, 1)
-template <int HD, int CT, bool PACK> struct Tile<EHIP_KV_Q4, HD, CT, PACK> {
+template <int HD, int CT, bool PACK, bool QL> struct Tile<EHIP_KV_Q4, HD, CT, PACK, QL> {
     static constexpr int NB = HD / QB, NP = HD / 64;
+    static constexpr int NH = PACK ? 1 : 2, QN = NB * NH;
     i32x4 k[NP], v[NP], ks[NB], vs[NB];
-    QHalf<HD, CT, PACK> Q;
+    i32x4 Q[QL ? 1 : CT][QN];
+    const i32x4 *ql;
     int E = 14;                  // the outputs' sums carry 2^E: 14, or 6 once a value was 4096 and more
     const uint8_t *kb, *vb;
     uint32_t magic;
@@ -277,8 +63,19 @@ template <int HD, int CT, bool PACK> struct Tile<EHIP_KV_Q4, HD, CT, PACK> {
         kb = a.kc + kv * a.head_bytes;
         vb = a.vc + kv * a.head_bytes;
     }
-    __device__ __forceinline__ void load_q(const AttendArgs &a, const float *row, int c, float &sc) {
-        load_q16<HD, CT, PACK, true>(a, row, c, Q, sc);
+    __device__ __forceinline__ void load_q(const AttendArgs &a, const float *row, int c, float &sc, i32x4 *lds) {
+        QHalf<HD, PACK> x;
+        load_q16<HD, PACK, true>(a, row, x, sc);
+#pragma unroll
+        for (int b = 0; b < QN / NH; b++)
+#pragma unroll
+            for (int h = 0; h < NH; h++) {
+                if (QL) lds[((c * QN) + b * NH + h) * 64 + (threadIdx.x & 63)] = x.q[b][h];
+                else Q[c][b * NH + h] = x.q[b][h];
+            }
+    }
+    __device__ __forceinline__ i32x4 q_at(int c, int b, int h) const {
+        return QL ? ql[(c * QN + b * NH + h) * 64 + (threadIdx.x & 63)] : Q[QL ? 0 : c][b * NH + h];
     }
     __device__ __forceinline__ void load_k(const AttendArgs &, int tile, int) {
         const int lane = threadIdx.x & 63, g = lane >> 4;
@@ -309,7 +106,7 @@ template <int HD, int CT, bool PACK> struct Tile<EHIP_KV_Q4, HD, CT, PACK> {
                 for (int c = 0; c < CT; c++) {
                     f32x4 x = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
-                    for (int h = 0; h < QHalf<HD, CT, PACK>::NH; h++) x = mfma16(codes, Q.q[c][b][h], x);
+                    for (int h = 0; h < NH; h++) x = mfma16(codes, q_at(c, b, h), x);
 #pragma unroll
                     for (int i = 0; i < 4; i++) S[c][s][i] = __builtin_fmaf(x[i], half_of(ks[b][i], s), S[c][s][i]);
                 }
@@ -426,18 +223,31 @@ __device__ __forceinline__ void odd_values(const AttendArgs &a, Rows<HD, CT> &R,
 // fp16: the lanes' pieces of K are 16-byte loads; a V operand is gathered from
 // 8 positions (64 bytes of a position to 16 lanes).  Positions past last_pos
 // repeat it.
-template <int HD, int CT, bool PACK> struct Tile<EHIP_KV_F16, HD, CT, PACK> {
+template <int HD, int CT, bool PACK, bool QL> struct Tile<EHIP_KV_F16, HD, CT, PACK, QL> {
     static constexpr int NB = (HD + 31) / 32;
+    static constexpr int NH = PACK ? 1 : 2, QN = NB * NH;
     i32x4 k[2][NB], v[HD / 16];
-    QHalf<HD, CT, PACK> Q;
+    i32x4 Q[QL ? 1 : CT][QN];
+    const i32x4 *ql;
     const _Float16 *kb, *vb;
 
     __device__ __forceinline__ void init(const AttendArgs &a, int kv) {
         kb = reinterpret_cast<const _Float16 *>(a.kc) + kv * HD;
         vb = reinterpret_cast<const _Float16 *>(a.vc) + kv * HD;
     }
-    __device__ __forceinline__ void load_q(const AttendArgs &a, const float *row, int c, float &sc) {
-        load_q16<HD, CT, PACK, false>(a, row, c, Q, sc);
+    __device__ __forceinline__ void load_q(const AttendArgs &a, const float *row, int c, float &sc, i32x4 *lds) {
+        QHalf<HD, PACK> x;
+        load_q16<HD, PACK, false>(a, row, x, sc);
+#pragma unroll
+        for (int b = 0; b < QN / NH; b++)
+#pragma unroll
+            for (int h = 0; h < NH; h++) {
+                if (QL) lds[((c * QN) + b * NH + h) * 64 + (threadIdx.x & 63)] = x.q[b][h];
+                else Q[c][b * NH + h] = x.q[b][h];
+            }
+    }
+    __device__ __forceinline__ i32x4 q_at(int c, int b, int h) const {
+        return QL ? ql[(c * QN + b * NH + h) * 64 + (threadIdx.x & 63)] : Q[QL ? 0 : c][b * NH + h];
     }
     __device__ __forceinline__ void load_k(const AttendArgs &a, int tile, int last_pos) {
         const int lane = threadIdx.x & 63, g = lane >> 4;
@@ -472,7 +282,7 @@ template <int HD, int CT, bool PACK> struct Tile<EHIP_KV_F16, HD, CT, PACK> {
 #pragma unroll
                 for (int b = 0; b < NB; b++)
 #pragma unroll
-                    for (int h = 0; h < QHalf<HD, CT, PACK>::NH; h++) S[c][s] = mfma16(k[s][b], Q.q[c][b][h], S[c][s]);
+                    for (int h = 0; h < NH; h++) S[c][s] = mfma16(k[s][b], q_at(c, b, h), S[c][s]);
                 if (PACK) S[c][s] = add_halves(S[c][s]);
             }
     }
@@ -490,7 +300,7 @@ template <int HD, int CT, bool PACK> struct Tile<EHIP_KV_F16, HD, CT, PACK> {
                     if (a1) v[d][i] &= 0x0000ffff;
                 }
         }
-        softmax_step(R, S, 1.0f);
+        softmax_step(R, S);
 #pragma unroll
         for (int c = 0; c < CT; c++) {
             i32x4 hi, lo;
@@ -509,24 +319,33 @@ template <int HD, int CT, bool PACK> struct Tile<EHIP_KV_F16, HD, CT, PACK> {
 // fp32, on the fp32 matrix cores (16x16x4): lane quarter g supplies dims
 // g HD / 4 .. of K and Q, so its pieces are contiguous; a P.V step contracts
 // one position per quarter.
-template <int HD, int CT, bool PACK> struct Tile<EHIP_KV_F32, HD, CT, PACK> {
+template <int HD, int CT, bool PACK, bool QL> struct Tile<EHIP_KV_F32, HD, CT, PACK, QL> {
     static_assert(!PACK, "fp32 rows have no low halves");
     static constexpr int NQ = HD / 16;   // 16-byte pieces of a quarter
-    f32x4 k[2][NQ], q[CT][NQ];
+    f32x4 k[2][NQ], q[QL ? 1 : CT][NQ];
     float v[HD / 16][2][4];
+    const i32x4 *ql;
     const float *kb, *vb;
 
     __device__ __forceinline__ void init(const AttendArgs &a, int kv) {
         kb = reinterpret_cast<const float *>(a.kc) + kv * HD;
         vb = reinterpret_cast<const float *>(a.vc) + kv * HD;
     }
-    __device__ __forceinline__ void load_q(const AttendArgs &a, const float *row, int c, float &sc) {
+    static constexpr int QN = NQ;
+    __device__ __forceinline__ void load_q(const AttendArgs &a, const float *row, int c, float &sc, i32x4 *lds) {
         const int g = (threadIdx.x & 63) >> 4;
 #pragma unroll
-        for (int j = 0; j < NQ; j++)
+        for (int j = 0; j < NQ; j++) {
+            f32x4 x;
 #pragma unroll
-            for (int r = 0; r < 4; r++) q[c][j][r] = row[g * (HD / 4) + 4 * j + r] * a.qscale;
+            for (int r = 0; r < 4; r++) x[r] = row[g * (HD / 4) + 4 * j + r] * a.qscale;
+            if (QL) reinterpret_cast<f32x4 *>(lds)[(c * NQ + j) * 64 + (threadIdx.x & 63)] = x;
+            else q[QL ? 0 : c][j] = x;
+        }
         sc = 1.0f;
+    }
+    __device__ __forceinline__ f32x4 q_at(int c, int j) const {
+        return QL ? reinterpret_cast<const f32x4 *>(ql)[(c * NQ + j) * 64 + (threadIdx.x & 63)] : q[QL ? 0 : c][j];
     }
     __device__ __forceinline__ void load_k(const AttendArgs &a, int tile, int last_pos) {
         const int lane = threadIdx.x & 63, g = lane >> 4;
@@ -555,9 +374,11 @@ template <int HD, int CT, bool PACK> struct Tile<EHIP_KV_F32, HD, CT, PACK> {
             for (int c = 0; c < CT; c++) {
                 S[c][s] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
-                for (int j = 0; j < NQ; j++)
+                for (int j = 0; j < NQ; j++) {
+                    const f32x4 x = q_at(c, j);
 #pragma unroll
-                    for (int r = 0; r < 4; r++) S[c][s] = __builtin_amdgcn_mfma_f32_16x16x4f32(k[s][j][r], q[c][j][r], S[c][s], 0, 0, 0);
+                    for (int r = 0; r < 4; r++) S[c][s] = __builtin_amdgcn_mfma_f32_16x16x4f32(k[s][j][r], x[r], S[c][s], 0, 0, 0);
+                }
             }
     }
     template <bool MASKED>
@@ -575,7 +396,7 @@ template <int HD, int CT, bool PACK> struct Tile<EHIP_KV_F32, HD, CT, PACK> {
                         if (bad) v[d][s][i] = 0.0f;
                     }
         }
-        softmax_step(R, S, 1.0f);
+        softmax_step(R, S);
 #pragma unroll
         for (int c = 0; c < CT; c++)
 #pragma unroll
@@ -589,41 +410,14 @@ template <int HD, int CT, bool PACK> struct Tile<EHIP_KV_F32, HD, CT, PACK> {
     __device__ __forceinline__ int exponent() const { return 0; }
 };
 
-// dims d .. d + 3 of row r of key head kv: o / l
-template <int HD>
-__device__ __forceinline__ void store_out(const AttendArgs &a, int pos0, int kv, int r, int d, f32x4 o, float l) {
-    const int b = r / a.G;
-    const float inv = 1.0f / l;
-    o *= inv;
-    if (pos0 + b < 0 || pos0 + b >= a.ctx) o = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
-    float *dst = a.out + (int64_t)b * a.out_stride + (kv * a.G + r % a.G) * HD + d;
-    if (a.out_vec) {
-        *reinterpret_cast<f32x4 *>(dst) = o;
-    } else {
-#pragma unroll
-        for (int j = 0; j < 4; j++) dst[j] = o[j];
-    }
-}
-
-// 16 bytes that workgroups of other XCDs read or have written: agent scope,
-// so they pass the XCD's L2 both ways (a release and acquire per workgroup
-// instead writes back and drops a whole L2 each time: 512 workgroups 17 us
-// where 264 take 12)
-__device__ __forceinline__ void put_part(float *p, f32x4 v) {
-    typedef unsigned long long u64x2 __attribute__((ext_vector_type(2)));
-    const u64x2 w = __builtin_bit_cast(u64x2, v);
-    unsigned long long *q = reinterpret_cast<unsigned long long *>(p);
-    __hip_atomic_store(q, w[0], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-    __hip_atomic_store(q + 1, w[1], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-}
-__device__ __forceinline__ f32x4 get_part(const float *p) {
-    typedef unsigned long long u64x2 __attribute__((ext_vector_type(2)));
-    const unsigned long long *q = reinterpret_cast<const unsigned long long *>(p);
-    const u64x2 w = u64x2{ __hip_atomic_load(q, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT), __hip_atomic_load(q + 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) };
-    return __builtin_bit_cast(f32x4, w);
-}
-
 // ---- the kernel ------------------------------------------------------------
+// Q in LDS, where the outputs go at the end, instead of in 64 registers: 32 rows
+// of 128 dims then leave room for two waves on a SIMD (16 heads of 128, 4096
+// tokens: 4 bits 305 -> 223 us, fp16 270 -> 211).  64 dims have two waves in
+// any case (4 bits, 14 heads and 4096 tokens 115 -> 129), and an fp32 tile
+// would spill (1024 tokens 61 -> 105).
+constexpr bool q_in_lds(int type, int hd, int ct) { return type != EHIP_KV_F32 && hd == 128 && ct == 2; }
+
 // Workgroup (unit, split): unit = (row group, key head), key heads fastest so
 // that a key head's workgroups share an XCD's L2; row groups from the last, so
 // that the longest start first.  The unit's nsplit workgroups take equal runs
@@ -631,12 +425,12 @@ __device__ __forceinline__ f32x4 get_part(const float *p) {
 // the tiles w, w + NW, ... of the run.  The last workgroup of a unit to arrive puts
 // the runs together.
 template <int TYPE, int HD, int CT, bool PACK, int NW>
-__global__ __launch_bounds__(64 * NW) void k_attend(AttendArgs a) {
+__device__ __forceinline__ void attend_body(const AttendArgs &a) {
     constexpr int BR = PACK ? 8 : 16 * CT;        // rows of a unit
     constexpr int LD = HD + 4;                    // floats between rows in LDS
     __shared__ __align__(16) float so[NW][BR][LD];
     __shared__ float sm[NW][BR], sl[NW][BR], ssc[BR], se[NW];
-    __shared__ int s_last;
+    static_assert(join_floats(BR, 64 * NW) * 4 <= sizeof(so), "the join fits the waves' outputs");
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, g = lane >> 4;
     const int nunits = gridDim.x / a.nsplit;
     const int unit = blockIdx.x % nunits, split = blockIdx.x / nunits;
@@ -652,7 +446,11 @@ __global__ __launch_bounds__(64 * NW) void k_attend(AttendArgs a) {
     const int v1 = min((split + 1) * run, ntiles);
 
     Rows<HD, CT> R;
-    Tile<TYPE, HD, CT, PACK> X;
+    constexpr bool QL = q_in_lds(TYPE, HD, CT);
+    Tile<TYPE, HD, CT, PACK, QL> X;
+    static_assert(CT * Tile<TYPE, HD, CT, PACK, QL>::QN * 1024 <= sizeof(so) && CT <= NW, "Q fits the outputs' place");
+    i32x4 *ql = reinterpret_cast<i32x4 *>(&so[0][0][0]);
+    X.ql = ql;
     X.init(a, kv);
     int vi = split * run + wave;
     if (vi < v1) {
@@ -667,11 +465,19 @@ __global__ __launch_bounds__(64 * NW) void k_attend(AttendArgs a) {
         R.l[c] = 0.0f;
 #pragma unroll
         for (int d = 0; d < HD / 16; d++) R.o[c][d] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
-        X.load_q(a, a.q + (int64_t)b * a.q_stride + (kv * a.G + r % a.G) * HD, c, R.sc[c]);
+        if (QL && wave != c) continue;
+        X.load_q(a, a.q + (int64_t)b * a.q_stride + (kv * a.G + r % a.G) * HD, c, R.sc[c], ql);
+        if (QL && g == 0) ssc[16 * c + lane] = R.sc[c];
+    }
+    if (QL) {
+        lds_barrier();
+#pragma unroll
+        for (int c = 0; c < CT; c++) R.sc[c] = ssc[16 * c + (lane & 15)];
     }
     // positions that every row sees: up to that of the first row, and from the last row's window on (or a sink)
     const int all_to = pos0 + r0 / a.G, all_from = a.window > 0 ? pos0 + (r1 - 1) / a.G - a.window + 1 : 0;
     while (vi < v1) {
+        if (QL) asm volatile("" ::: "memory");   // (Q stays in LDS: the compiler would keep it in registers over the loop)
         const int tile = T.at(vi), t0 = tile * KV_TILE;
         const bool whole = t0 + KV_TILE - 1 <= all_to && (t0 >= all_from || t0 + KV_TILE <= a.sinks);
         f32x4 S[CT][2];
@@ -686,6 +492,7 @@ __global__ __launch_bounds__(64 * NW) void k_attend(AttendArgs a) {
         }
         if (vi < v1) X.load_v(a, T.at(vi), last_pos);
     }
+    if (QL) lds_barrier();   // (every wave is past its last reads of Q)
 
     // ---- the workgroup's waves: a row's sums weigh 2^((m - M) sc), M the largest of its m, the output's 2^-E of it
     const int E = X.exponent();
@@ -708,7 +515,7 @@ __global__ __launch_bounds__(64 * NW) void k_attend(AttendArgs a) {
     if (lane == 0) se[wave] = __builtin_amdgcn_ldexpf(1.0f, -E);
     __syncthreads();
     const bool alone = nact == 1;
-    const int64_t slot = (int64_t)unit * a.nsplit + split;
+    const Parts<HD, BR> mine(a, (int64_t)unit * a.nsplit + split, 1);
     for (int i = tid; i < BR * (HD / 4); i += 64 * NW) {
         const int r = i / (HD / 4), d = i % (HD / 4) * 4;
         float M = sm[0][r];
@@ -726,89 +533,89 @@ __global__ __launch_bounds__(64 * NW) void k_attend(AttendArgs a) {
         if (alone) {
             store_out<HD>(a, pos0, kv, r0 + r, d, o, l);
         } else {
-            put_part(a.part + (slot * BR + r) * HD + d, o);
-            if (d == 0) put_part(reinterpret_cast<float *>(a.part_ml + slot * BR + r), f32x4{M, l, ssc[r], 0.0f});
+            mine.rows.put((r * HD + d) * 4, o);
+            if (d == 0) mine.ml.put(r * 16, f32x4{M, l, ssc[r], 0.0f});
         }
     }
     if (alone) return;
 
-    // ---- the unit's workgroups: the last one to arrive joins the runs.  Every
-    // wave's partial stores have completed, past its XCD's L2, before the
-    // workgroup counts itself, and the last one's loads go past its own.
-    __builtin_amdgcn_s_waitcnt(0);
-    __syncthreads();
-    if (tid == 0) s_last = __hip_atomic_fetch_add(a.count + unit, 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == nact - 1;
-    __syncthreads();
-    if (!s_last) return;
-    if (tid == 0) __hip_atomic_store(a.count + unit, 0, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-    const int64_t base = (int64_t)unit * a.nsplit;
-    float *sf = &so[0][0][0];                       // [row][AT_SPLITS]: the runs' weights over the row's sum
-    f32x4 *red = reinterpret_cast<f32x4 *>(sf + BR * AT_SPLITS);
-    static_assert(BR * AT_SPLITS * 4 + 64 * NW * 16 <= sizeof(so), "the join fits the waves' outputs");
-    const int nr = r1 - r0;
-    for (int r = wave; r < nr; r += NW) {     // a wave a row, a lane a run: one round trip
-        const f32x4 ml = get_part(reinterpret_cast<const float *>(a.part_ml + (base + min(lane, nact - 1)) * BR + r));
-        const float m = lane < nact ? ml[0] : -INFINITY, M = wave_max(m);
-        const float f = m == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f((m - M) * ml[2]);
-        const float l = wave_sum(lane < nact ? f * ml[1] : 0.0f);
-        sf[r * AT_SPLITS + lane] = f;
-        if (lane == 0) sl[0][r] = l;
-    }
-    __syncthreads();
-    // an item is four dims of a row; with fewer items than threads they share the runs
-    const int items = nr * (HD / 4), parts = max(64 * NW / items, 1);
-    for (int i0 = 0; i0 < items; i0 += 64 * NW) {
-        const int part = parts > 1 ? tid / items : 0, i = parts > 1 ? tid % items : i0 + tid;
-        const int r = min(i, items - 1) / (HD / 4), d = i % (HD / 4) * 4;
-        f32x4 o = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
-        if (i < items && part < parts) {
-            const float *p = a.part + (base * BR + r) * HD + d;
-            for (int z = part; z < nact; z += 8 * parts) {
-                f32x4 x[8];
-#pragma unroll
-                for (int j = 0; j < 8; j++) x[j] = get_part(p + (int64_t)min(z + j * parts, nact - 1) * (BR * HD));
-#pragma unroll
-                for (int j = 0; j < 8; j++) {
-                    const float f = z + j * parts < nact ? sf[r * AT_SPLITS + z + j * parts] : 0.0f;
-                    o += x[j] * f;
-                }
-            }
-        }
-        if (parts > 1) {
-            red[tid] = o;
-            __syncthreads();
-            if (tid >= items) return;
-            for (int q = 1; q < parts; q++) o += red[q * items + tid];
-        }
-        if (i < items) store_out<HD>(a, pos0, kv, r0 + r, d, o, sl[0][r]);
-    }
+    join_runs<HD, BR, 64 * NW>(a, unit, nact, r0, r1, pos0, kv, &so[0][0][0]);
 }
+
+template <int TYPE, int HD, int CT, bool PACK, int NW>
+__global__ __launch_bounds__(64 * NW) void k_attend(AttendArgs a) { attend_body<TYPE, HD, CT, PACK, NW>(a); }
+// the same held to the registers of two waves on a SIMD
+template <int TYPE, int HD, int CT, bool PACK, int NW>
+__global__ __launch_bounds__(64 * NW, 2) void k_attend_two(AttendArgs a) { attend_body<TYPE, HD, CT, PACK, NW>(a); }
 
 // ---- shapes of a launch ------------------------------------------------------
 // Rows of a unit: 8 (PACK) or 16 while they hold all the rows of a key head,
-// else 32.  Waves of a workgroup: 4; for few rows of a 4-bit cache 8 where 4
-// would make more workgroups than CUs, as half the ranges are then joined
-// (16 heads of 128 over 8192 positions 15.0 -> 13.4 us; over 2048, which 4
-// waves spread over more CUs, 10.0 -> 10.9; an fp32 cache, whose products are
-// longer, 54 -> 58 over 32,768).
-struct Shape { int br, waves; int64_t units; int nsplit; };
-static Shape shape_of(const EhipCache &c, int n_heads, int n_tok, int64_t tiles) {
-    Shape s;
-    const int64_t rows = (int64_t)n_tok * (n_heads / c.n_kv);
-    s.br = c.type != EHIP_KV_F32 && rows <= 8 ? 8 : rows <= 16 ? 16 : 32;
-    s.units = (rows + s.br - 1) / s.br * c.n_kv;
-    s.waves = c.type == EHIP_KV_Q4 && s.br <= 16 && s.units * ((tiles + 3) / 4) > 256 ? 8 : 4;
-    // 2048 waves (two to each SIMD), each with at least a tile
-    const int64_t all = 2048 / s.waves, want = s.units >= all ? 1 : (all + s.units - 1) / s.units, most = (tiles + s.waves - 1) / s.waves;
-    s.nsplit = (int)(want < most ? want : most);
-    if (s.nsplit > AT_SPLITS) s.nsplit = AT_SPLITS;
+// then 32; over an fp32 cache ATTEND_ROWS (attend_rows.hip), if that makes four
+// tiles and more for each workgroup that the GPU holds: 16 heads of 128, whole
+// prompts, 512 tokens 36 us (48 there), 1024 61 (64), 2048 183 (129).  Waves of
+// a workgroup: 4; for few rows of a 4-bit cache 8 where 4 would make more
+// workgroups than CUs, as half the ranges are then joined (16 heads of 128 over
+// 8192 positions 15.0 -> 13.4 us; over 2048, which 4 waves spread over more
+// CUs, 10.0 -> 10.9; an fp32 cache, whose products are longer, 54 -> 58 over
+// 32,768).
+struct Shape { int br, waves; int64_t units; int nsplit, run; };
+constexpr int SLOTS = 512;       // workgroups of four waves that the GPU holds, two waves to each SIMD
+constexpr int MAX_UNITS = 2 * SLOTS;   // units from which on none is split
+
+static int tiles_of_rows(int64_t pos0, int64_t r0, int64_t r1, int G, int window, int sinks) {
+    return tiles_seen((int)(pos0 + r0 / G), (int)(pos0 + (r1 - 1) / G), window, sinks).n;
+}
+
+static int few_rows(int type, int64_t rows) { return type != EHIP_KV_F32 && rows <= 8 ? 8 : rows <= 16 ? 16 : 32; }
+
+// q: its n_tok, n_heads, window and sinks; positions: q.pos0, or any (q.pos)
+static Shape shape_of(const EhipCache &c, const EhipAttend &q) {
+    Shape s{};
+    const int G = q.n_heads / c.n_kv;
+    const int64_t rows = (int64_t)q.n_tok * G;
+    const int64_t pos0 = q.pos ? c.ctx - q.n_tok : q.pos0;
+    s.br = few_rows(c.type, rows);
+    int tiles = 0;
+    int64_t all = 0;             // many rows: tiles of all units
+    if (c.type == EHIP_KV_F32 && rows >= ATTEND_ROWS) {
+        for (int64_t r = 0; r < rows; r += ATTEND_ROWS) {   // (behind a window a last group of few rows sees less than one before)
+            const int n = tiles_of_rows(pos0, r, r + ATTEND_ROWS < rows ? r + ATTEND_ROWS : rows, G, q.window, q.sinks);
+            all += (int64_t)n * c.n_kv;
+            if (n > tiles) tiles = n;
+        }
+        if (all >= 4 * SLOTS) s.br = ATTEND_ROWS;
+    }
+    const int64_t groups = (rows + s.br - 1) / s.br;
+    s.units = groups * c.n_kv;
+    s.waves = 4;
+    if (s.br == ATTEND_ROWS) {
+        // ranges of a slot's average, of at least 8 tiles (a range's start and
+        // its join take the time of about four)
+        int64_t run = (all + SLOTS - 1) / SLOTS;
+        if (run < 8) run = 8;
+        // many units fill the slots by themselves, and a rest of less than a
+        // quarter is not worth a join
+        if (s.units >= MAX_UNITS || tiles <= run + run / 4) run = tiles;
+        s.nsplit = (int)((tiles + run - 1) / run);
+        s.run = q.pos ? 0 : (int)run;
+    } else {
+        tiles = tiles_of_rows(pos0, (groups - 1) * s.br, rows, G, q.window, q.sinks);
+        if (c.type == EHIP_KV_Q4 && s.br <= 16 && s.units * ((tiles + 3) / 4) > 256) s.waves = 8;
+        // two waves to each SIMD, each with at least a tile
+        const int64_t most = (tiles + s.waves - 1) / s.waves, slots = SLOTS * 4 / s.waves, want = s.units >= slots ? 1 : (slots + s.units - 1) / s.units;
+        s.nsplit = (int)(want < most ? want : most);
+    }
+    if (s.nsplit > AT_SPLITS) {
+        s.nsplit = AT_SPLITS;
+        if (s.run) s.run = (tiles + AT_SPLITS - 1) / AT_SPLITS;
+    }
     if (s.nsplit < 1) s.nsplit = 1;
     return s;
 }
 
-// Workspace: the units' counters (units that split are fewer than 512), then
-// the partial rows and their (maximum, sum).
-constexpr int COUNT_BYTES = 2048;
+// Workspace: the units' counters (units that split are fewer than MAX_UNITS),
+// then the partial rows and their (maximum, sum, scale).
+constexpr int COUNT_BYTES = 4 * MAX_UNITS;
 static uint64_t space_bytes(int64_t rows, int hd) { return rows ? COUNT_BYTES + (uint64_t)rows * (4 * hd + 16) : 0; }
 static int64_t space_rows(const Shape &s) { return s.nsplit > 1 ? s.units * s.nsplit * s.br : 0; }
 
@@ -823,21 +630,18 @@ static int attend_go(hipStream_t st, const AttendArgs &a, const Shape &s) {
         if (s.br == 16 && s.waves == 8) hipLaunchKernelGGL((k_attend<TYPE, HD, 1, false, 8>), grid, wg, 0, st, a);
     }
     if (s.br == 16 && s.waves == 4) hipLaunchKernelGGL((k_attend<TYPE, HD, 1, false, 4>), grid, wg, 0, st, a);
-    else if (s.br == 32) hipLaunchKernelGGL((k_attend<TYPE, HD, 2, false, 4>), grid, wg, 0, st, a);
+    if (s.br == 32) {
+        if constexpr (q_in_lds(TYPE, HD, 2)) hipLaunchKernelGGL((k_attend_two<TYPE, HD, 2, false, 4>), grid, wg, 0, st, a);
+        else hipLaunchKernelGGL((k_attend<TYPE, HD, 2, false, 4>), grid, wg, 0, st, a);
+    }
+    if (TYPE == EHIP_KV_F32 && s.br == ATTEND_ROWS) launch_attend_rows(st, HD, s.units * s.nsplit, a);
     const hipError_t e = hipGetLastError();
     return e == hipSuccess ? 0 : refuse("ehip_attend: launch: %s", hipGetErrorString(e));
 }
 
 // How a call is shared over workgroups; -1 where its workspace does not do.
 static int shape_call(const EhipCache &c, const EhipAttend &q, Shape *s) {
-    // a host position says how many tiles there are to share
-    int64_t tiles = (c.ctx + KV_TILE - 1) / KV_TILE;
-    if (!q.pos) tiles = ((int64_t)q.pos0 + q.n_tok + KV_TILE - 1) / KV_TILE;
-    if (q.window > 0) {
-        const int64_t in = ((int64_t)q.window + q.n_tok + 2 * KV_TILE) / KV_TILE + ((int64_t)q.sinks + KV_TILE - 1) / KV_TILE;
-        if (in < tiles) tiles = in;
-    }
-    *s = shape_of(c, q.n_heads, q.n_tok, tiles);
+    *s = shape_of(c, q);
     const uint64_t need = space_bytes(space_rows(*s), c.head_dim);
     if (need && (!q.workspace || !aligned(q.workspace, 16) || q.workspace_bytes < need))
         return refuse("ehip_attend: the workspace is null, not 16-byte aligned, or smaller than this call's %llu bytes", (unsigned long long)need);
@@ -847,6 +651,7 @@ static int shape_call(const EhipCache &c, const EhipAttend &q, Shape *s) {
 int launch_attend(hipStream_t st, const EhipCache &c, const EhipAttend &q) {
     Shape s;
     if (shape_call(c, q, &s)) return -1;
+    if (!q.q || !q.out) return refuse("ehip_attend: null rows");
     AttendArgs a{};
     a.q = q.q; a.out = q.out; a.q_stride = q.q_stride; a.out_stride = q.out_stride;
     a.kc = static_cast<const uint8_t *>(c.k); a.vc = static_cast<const uint8_t *>(c.v);
@@ -856,6 +661,7 @@ int launch_attend(hipStream_t st, const EhipCache &c, const EhipAttend &q) {
     a.window = q.window; a.sinks = q.sinks;
     a.qscale = (q.scale != 0.0f ? q.scale : 1.0f / sqrtf((float)c.head_dim)) * 1.4426950408889634f;
     a.nsplit = s.nsplit;
+    a.run = s.run;
     a.out_vec = aligned(q.out, 16) && q.out_stride % 4 == 0;
     if (s.nsplit > 1) {
         a.count = static_cast<int *>(q.workspace);
@@ -892,16 +698,22 @@ extern "C" uint64_t ehip_attend_workspace(const EhipCache *c, int n_heads, int n
     const int G = n_heads / c->n_kv;
     const int64_t tiles = (c->ctx + KV_TILE - 1) / KV_TILE;
     uint64_t most = 0;
-    // on the way to n_tok tokens a unit's rows go through at most three sizes:
-    // the largest counts of tokens of each, with either count of waves
-    for (int64_t n : { (int64_t)1, (int64_t)8 / G, (int64_t)16 / G, (int64_t)n_tok }) {
-        if (n < 1 || n > n_tok) continue;
-        const Shape s = shape_of(*c, n_heads, (int)n, tiles);
-        const int64_t all = 512, units = s.units < all - 1 ? s.units : all - 1, by_tiles = units * ((tiles + 3) / 4);
-        const int64_t wgs = all - 1 + units < by_tiles ? all - 1 + units : by_tiles;
-        const uint64_t b = wgs > units ? space_bytes(wgs * s.br, c->head_dim) : 0;
+    // On the way to n_tok tokens a unit's rows go through at most four sizes;
+    // the largest count of tokens of each, U units of it and T tiles at most.
+    // Few rows: at most SLOTS - 1 + U workgroups.  Many: tiles per unit grow
+    // along a prompt ever more slowly, so the average is at least half of the
+    // most, and with it a range: U (2 SLOTS / U + 1), and U more for rounding.
+    auto bound = [&](int64_t rows, int br) {
+        const bool many = br == ATTEND_ROWS;
+        const int64_t units = (rows + br - 1) / br * c->n_kv, top = many ? MAX_UNITS - 1 : SLOTS - 1, U = units < top ? units : top;
+        const int64_t wgs = many ? 2 * SLOTS + 2 * U : SLOTS - 1 + U, by_tiles = U * ((tiles + (many ? 7 : 3)) / (many ? 8 : 4));
+        const uint64_t b = by_tiles > U ? space_bytes((wgs < by_tiles ? wgs : by_tiles) * br, c->head_dim) : 0;
         if (b > most) most = b;
-    }
+    };
+    const int64_t all = (int64_t)n_tok * G;
+    for (int64_t rows : { (int64_t)G, (int64_t)8 / G * G, (int64_t)16 / G * G, all })
+        if (rows > 0 && rows <= all) bound(rows, few_rows(c->type, rows));
+    if (c->type == EHIP_KV_F32 && all >= ATTEND_ROWS) bound(all, ATTEND_ROWS);
     return most;
 }
 
@@ -917,8 +729,5 @@ extern "C" int ehip_attend(const EhipCache *c, const EhipAttend *q, void *stream
     if (!(q->scale - q->scale == 0.0f)) return refuse("%s: scale %g", who, (double)q->scale);
     if (!q->pos && (q->pos0 < 0 || (int64_t)q->pos0 + q->n_tok > c->ctx))
         return refuse("%s: positions %d..%lld exceed the cache of %lld", who, q->pos0, (long long)q->pos0 + q->n_tok - 1, (long long)c->ctx);
-    Shape s;
-    if (shape_call(*c, *q, &s)) return -1;
-    if (!q->q || !q->out) return refuse("%s: null rows", who);
     return launch_attend(static_cast<hipStream_t>(stream), *c, *q);
 }

@@ -245,7 +245,7 @@ typedef struct {
     float          scale;                 /* 0: 1 / sqrt(head_dim)                   */
     const int32_t *pos;                   /* the first token's position, or NULL     */
     void          *workspace;             /* ehip_attend_workspace bytes, 16-byte aligned,
-                                             its first 2048 zero before its first call;
+                                             its first 4096 zero before its first call;
                                              calls that may run at the same time need
                                              one each                                 */
     uint64_t       workspace_bytes;

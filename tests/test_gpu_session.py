@@ -305,7 +305,7 @@ def attend(c, q, pos0, window=0, sinks=0, scale=0.0, pos=None, stride=None, stre
                            sinks=sinks, scale=scale, pos=pos, workspace=ws.ptr, workspace_bytes=ws.nbytes)
     ok(lib.ehip_attend(c.c, a, stream))
     R.hip().sync()
-    assert not ws.nbytes or not ws.read()[:2048].any()   # the counters are zero again
+    assert not ws.nbytes or not ws.read()[:4096].any()   # the counters are zero again
     flat = out.read()
     assert untouched(flat, n, w, stride)
     return as_rows(flat, n, w, stride).reshape(n, nh, hd)
@@ -426,6 +426,74 @@ def test_attend_strides_positions_streams_and_workspaces(kind, hd):
                 check_attend(got[i:i + 1], c, q[i:i + 1], k, v, p + i)
             else:
                 assert (got[i] == 0).all()
+    R.hip().h.hipStreamDestroy(stream)
+
+
+# Many rows over an fp32 cache: units of 128 rows, of 2048 tiles and more over
+# all units.  (n, pos0, window, sinks, heads of a key head, key heads)
+MANY = [(1, 1100, 0, 0, 4096, 2), (900, 0, 0, 0, 3, 8), (2200, 0, 0, 0, 1, 4), (333, 777, 0, 0, 7, 5), (130, 0, 16, 1, 512, 2), (64, 60, 1, 0, 1400, 3),
+        (130, 300, 100, 64, 256, 2), (200, 1000, 777, 33, 8, 8), (130, 0, 40, 0, 515, 2)]
+
+
+@pytest.mark.parametrize("hd", [48, 64, 128])
+@pytest.mark.parametrize("n,pos0,window,sinks,G,n_kv", MANY)
+def test_attend_many_rows_of_fp32(hd, n, pos0, window, sinks, G, n_kv):
+    c, k, v, rng = filled(F32, hd, n_kv, pos0 + n, pos0 + n + 3, n + window)
+    q = rng.standard_normal((n, G * n_kv, hd)).astype(np.float32)
+    check_attend(attend(c, q, pos0, window, sinks), c, q, k, v, pos0, window, sinks)
+
+
+@pytest.mark.parametrize("hd", [48, 64, 128])
+@pytest.mark.parametrize("n,pos0,window,sinks,bad,G", [(70, 64, 0, 0, (100, 130), 1000), (70, 200, 20, 3, (150, 231, 3), 2000)])
+def test_attend_many_rows_read_only_what_they_see(hd, n, pos0, window, sinks, bad, G):
+    c, k, v, rng = filled(F32, hd, 1, pos0 + n, pos0 + n + 40, n)
+    q = rng.standard_normal((n, G, hd)).astype(np.float32)
+    kb, vb = k.copy(), v.copy()
+    for i, b in enumerate(bad):
+        kb[b] = (np.nan, np.inf, -np.inf)[i % 3]
+        vb[b, 0, ::3] = (np.inf, np.nan, -np.inf)[i % 3]
+    c.store(kb, vb, 0)
+    p = pos0 + np.arange(n)
+    sees = np.zeros(n, bool)
+    for b in bad:
+        sees |= (b <= p) & ((b > p - window) | (b < sinks) if window else True)
+    assert sees.any() and not sees.all()
+    got = attend(c, q, pos0, window, sinks)
+    assert not np.isfinite(got[sees]).all(-1).any()
+    want, bound = R.attended(q, k.astype(np.float64), v.astype(np.float64), pos0, window, sinks)
+    within(np.abs(got - want)[~sees], bound[~sees])
+
+
+@pytest.mark.parametrize("hd", [64, 128])
+def test_attend_scales_of_many_rows(hd):
+    c, k, v, rng = filled(F32, hd, 1, 400, 400, 9)
+    v = (v * np.exp2(rng.integers(-12, 9, (400, 1, 1)))).astype(np.float32)
+    v[:64] *= np.float32(1e-3)
+    c.store(k, v, 0)
+    q = rng.standard_normal((64, 360, hd)).astype(np.float32)
+    for f in (0.0, 1e-30, 1e-3, 1.0, 12.0):
+        check_attend(attend(c, q * np.float32(f), 300), c, q * np.float32(f), k, v, 300)
+    for scale in (-0.07, 0.5):
+        check_attend(attend(c, q, 300, scale=scale), c, q, k, v, 300, scale=scale)
+
+
+@pytest.mark.parametrize("hd", [48, 128])
+def test_attend_strides_and_positions_of_many_rows(hd):
+    c, k, v, rng = filled(F32, hd, 2, 330, 330, 2)
+    stream = R.hip().stream()
+    n, heads = 20, 2 * 650
+    q = rng.standard_normal((n, heads, hd)).astype(np.float32)
+    want = attend(c, q, 300)
+    check_attend(want, c, q, k, v, 300)
+    np.testing.assert_array_equal(attend(c, q, 300, stride=heads * hd + 12), want)
+    np.testing.assert_array_equal(attend(c, q, 300, stride=heads * hd + 5, shift=1, stream=stream), want)
+    for p in (300, 100, 3, 0, 320, 329, 330, 5000, -7, -20, -2 ** 31, 2 ** 31 - 1):
+        pos = R.Buf(np.array([p], np.int32))
+        got = attend(c, q, 0, pos=pos.ptr)
+        a, b = max(0, -p), max(0, min(n, 330 - p))
+        if a < b:
+            check_attend(got[a:b], c, q[a:b], k, v, p + a)
+        assert (got[:min(a, n)] == 0).all() and (got[max(b, 0):] == 0).all()
     R.hip().h.hipStreamDestroy(stream)
 
 

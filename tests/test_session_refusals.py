@@ -125,8 +125,8 @@ def test_attend_refuses():
     assert L.ehip_attend(cache(), call(n_tok=0, q=None), None) == 0
     big = cache(ctx=4096)   # shared by workgroups: a workspace is needed
     need = L.ehip_attend_workspace(big, 4, 2)
-    assert need > 2048
-    for kw in (dict(), dict(workspace=P), dict(workspace=P, workspace_bytes=2048), dict(workspace=P + 8, workspace_bytes=need)):
+    assert need > 4096
+    for kw in (dict(), dict(workspace=P), dict(workspace=P, workspace_bytes=4096), dict(workspace=P + 8, workspace_bytes=need)):
         refused(L.ehip_attend(big, call(pos0=4000, **kw), None), "workspace")
 
 
