@@ -11,9 +11,9 @@
 // positions it does not store.
 //
 // Bound: memory.  A workgroup takes one tile of one key head: a thread's piece
-// of a key is 8 consecutive dims (its block's maximum over the 4 threads of the
-// block, a quad of lanes), a value's thread one dim of 8 positions (each
-// position's maximum over the 32 lanes of the block).
+// of a row is 8 consecutive dims (its block's maximum over the 4 threads of the
+// block, a quad of lanes); values' codes then cross over through LDS, 8
+// positions of 8 dims at a time.
 #include "session.h"
 
 namespace ehip {
@@ -49,99 +49,129 @@ __device__ __forceinline__ uint32_t q4_code(float x, float inv) {
     return (uint32_t)min(max(c, 0), 15);
 }
 
+// four floats of a row (rows of any alignment)
+typedef float RowV __attribute__((ext_vector_type(4), aligned(4)));
+
+// The codes of 8 dims of a row (nibble j: dim j) and their block's scale, the
+// block's other dims in the quad's other lanes.
+__device__ __forceinline__ uint32_t q4_piece(const RowV (&x)[2], uint16_t &d) {
+    uint32_t m = __float_as_uint(x[0][0]);
+#pragma unroll
+    for (int j = 1; j < 8; j++) m = q4_top(m, __float_as_uint(x[j / 4][j % 4]), false);
+    m = q4_top(m, (uint32_t)__builtin_amdgcn_mov_dpp((int)m, 0xb1, 0xf, 0xf, false), (threadIdx.x & 1) != 0);
+    m = q4_top(m, (uint32_t)__builtin_amdgcn_mov_dpp((int)m, 0x4e, 0xf, 0xf, false), (threadIdx.x & 2) != 0);
+    const Q4Scale s = q4_scale(m);
+    uint32_t w = 0;
+#pragma unroll
+    for (int j = 0; j < 8; j++) w |= q4_code(x[j / 4][j % 4], s.inv) << (4 * j);
+    d = s.d;
+    return w;
+}
+
+// nibble j of r[n] <-> nibble n of r[j]
+__device__ __forceinline__ void transpose_nibbles(uint32_t (&r)[8]) {
+#pragma unroll
+    for (int n = 0; n < 4; n++) {
+        const uint32_t a = r[n], b = r[n + 4];
+        r[n] = __builtin_amdgcn_perm(b, a, 0x05040100);
+        r[n + 4] = __builtin_amdgcn_perm(b, a, 0x07060302);
+    }
+#pragma unroll
+    for (int n = 0; n < 8; n += 1 + (n & 1) * 2) {   // 0, 1, 4, 5
+        const uint32_t a = r[n], b = r[n + 2];
+        r[n] = __builtin_amdgcn_perm(b, a, 0x06020400);
+        r[n + 2] = __builtin_amdgcn_perm(b, a, 0x07030501);
+    }
+#pragma unroll
+    for (int n = 0; n < 8; n += 2) {
+        const uint32_t a = r[n], b = r[n + 1];
+        r[n] = (a & 0x0f0f0f0fu) | (b & 0x0f0f0f0fu) << 4;
+        r[n + 1] = (a >> 4 & 0x0f0f0f0fu) | (b & 0xf0f0f0f0u);
+    }
+}
+
 // grid (tiles the tokens touch, n_kv)
 template <int HD>
 __global__ __launch_bounds__(WG) void k_kv4_store(KvArgs a) {
+    constexpr int NB = HD / QB, KP = HD / 8, KU = KV_TILE * KP / WG;
+    __shared__ uint32_t vc[KV_TILE][KP];
     const int tid = threadIdx.x, kv = blockIdx.y;
     const int64_t p0 = a.pos ? (int64_t)*a.pos : a.pos0;
     const int64_t first = p0 < 0 ? 0 : p0, end = min(p0 + a.n_tok, a.ctx);   // positions that are stored
     const int64_t tile = first / KV_TILE + blockIdx.x, t0 = tile * KV_TILE;
-    if (t0 >= end) return;
+    if (max(first, t0) >= end) return;
+    const int k0 = (int)max(first - t0, (int64_t)0), k1 = (int)min(end - t0, (int64_t)KV_TILE);   // those of this tile
     uint8_t *kt = a.kc + ((int64_t)kv * a.tiles + tile) * kv_tile_bytes(HD), *vt = a.vc + ((int64_t)kv * a.tiles + tile) * kv_tile_bytes(HD);
-    constexpr int NB = HD / QB;
-    const float *kr = a.k + (int64_t)kv * HD, *vr = a.v + (int64_t)kv * HD;
+    const float *kr = a.k + (t0 - p0) * a.k_stride + (int64_t)kv * HD, *vr = a.v + (t0 - p0) * a.v_stride + (int64_t)kv * HD;
 
-    // keys: thread (key, piece of 8 dims), pieces fastest
-    constexpr int KP = HD / 8;
+    // thread (position, piece of 8 dims), pieces fastest; all of its rows' loads
+    // are on their way before the first is used
+    RowV x[KU][2], y[KU][2];
 #pragma unroll
-    for (int u = 0; u < KV_TILE * KP / WG; u++) {
-        const int i = tid + u * WG, key = i / KP, c = i % KP, b = c / 4, g = c % 4;
-        const int64_t t = t0 + key;
-        const bool in = t >= first && t < end;
-        const float *src = kr + ((in ? t : max(first, t0)) - p0) * a.k_stride + 8 * c;   // (a stored position in any case)
-        float x[8];
+    for (int u = 0; u < KU; u++) {
+        const int i = tid + u * WG, t = min(max(i / KP, k0), k1 - 1), c = i % KP;   // (a stored position in any case)
+        const RowV *xs = reinterpret_cast<const RowV *>(kr + t * a.k_stride + 8 * c), *ys = reinterpret_cast<const RowV *>(vr + t * a.v_stride + 8 * c);
+        x[u][0] = xs[0]; x[u][1] = xs[1];
+        y[u][0] = ys[0]; y[u][1] = ys[1];
+    }
 #pragma unroll
-        for (int j = 0; j < 8; j++) x[j] = src[j];
-        uint32_t m = __float_as_uint(x[0]);
-#pragma unroll
-        for (int j = 1; j < 8; j++) m = q4_top(m, __float_as_uint(x[j]), false);
-#pragma unroll
-        for (int off = 1; off < 4; off <<= 1) m = q4_top(m, (uint32_t)__shfl_xor((int)m, off), (tid & off) != 0);
-        const Q4Scale s = q4_scale(m);
-        uint32_t w = 0;
-#pragma unroll
-        for (int j = 0; j < 8; j++) w |= q4_code(x[j], s.inv) << (4 * j);
-        if (in) {
-            const int half = key / 16, l = key % 16;
-            *reinterpret_cast<uint32_t *>(kt + kv_code_at(g * 16 + l, half * NB + b)) = w;
-            if (g == 0) *reinterpret_cast<uint16_t *>(kt + kv_scale_at(HD, l / 4, b, l % 4, half)) = s.d;
+    for (int u = 0; u < KU; u++) {
+        const int i = tid + u * WG, t = i / KP, c = i % KP, b = c / 4, g = c % 4, half = t / 16, l = t % 16;
+        const bool in = t >= k0 && t < k1;
+        uint16_t kd, vd;
+        const uint32_t kw = q4_piece(x[u], kd);
+        vc[t][c] = q4_piece(y[u], vd);
+        if (!in) continue;
+        *reinterpret_cast<uint32_t *>(kt + kv_code_at(g * 16 + l, half * NB + b)) = kw;
+        if (g == 0) {
+            *reinterpret_cast<uint16_t *>(kt + kv_scale_at(HD, l / 4, b, l % 4, half)) = kd;
+            *reinterpret_cast<uint16_t *>(vt + kv_scale_at(HD, l / 4, b, l % 4, half)) = vd;
         }
     }
+    __syncthreads();
 
-    // values: thread (quarter g, dim), dims fastest: positions 16 s + 4 g + i
-#pragma unroll 1
-    for (int u = 0; u < 4 * HD / WG; u++) {
-        const int j = tid + u * WG, dim = j % HD, g = j / HD, b = dim / QB;
-        uint32_t *dst = reinterpret_cast<uint32_t *>(vt + kv_code_at(g * 16 + dim % 16, dim / 16));
-        uint32_t w = 0, keep = 0;
-        uint16_t d[8];
-        float x[8];
+    // values: thread (quarter g, piece of 8 dims): positions 16 s + 4 g + i
+    if (tid >= 4 * KP) return;
+    const int g = tid / KP, c = tid % KP;
+    uint32_t keep = 0, r[8];
 #pragma unroll
-        for (int n = 0; n < 8; n++) {
-            const int64_t t = t0 + 16 * (n / 4) + 4 * g + n % 4;
-            const bool in = t >= first && t < end;
-            x[n] = in ? vr[(t - p0) * a.v_stride + dim] : 0.0f;
-            if (!in) keep |= 15u << (4 * n);
-        }
-#pragma unroll
-        for (int n = 0; n < 8; n++) {
-            uint32_t m = __float_as_uint(x[n]);
-#pragma unroll
-            for (int off = 1; off < 32; off <<= 1) m = q4_top(m, (uint32_t)__shfl_xor((int)m, off), (tid & off) != 0);
-            const Q4Scale s = q4_scale(m);
-            d[n] = s.d;
-            w |= q4_code(x[n], s.inv) << (4 * n);
-        }
-        if (keep == 0xffffffffu) continue;
-        if (keep) w = (w & ~keep) | (*dst & keep);
-        *dst = w;
-        if (dim % QB == 0) {
-#pragma unroll
-            for (int n = 0; n < 8; n++)
-                if (!(keep >> (4 * n) & 1)) *reinterpret_cast<uint16_t *>(vt + kv_scale_at(HD, g, b, n % 4, n / 4)) = d[n];
-        }
+    for (int n = 0; n < 8; n++) {
+        const int t = 16 * (n / 4) + 4 * g + n % 4;
+        if (t < k0 || t >= k1) keep |= 15u << (4 * n);
+        r[n] = vc[t][c];
     }
+    if (keep == 0xffffffffu) return;
+    transpose_nibbles(r);
+    uint8_t *dst = vt + kv_code_at(g * 16 + 8 * c % 16, c / 2);
+    if (keep) {
+        uint32_t old[8];
+#pragma unroll
+        for (int j = 0; j < 8; j++) old[j] = *reinterpret_cast<const uint32_t *>(dst + 16 * j);
+#pragma unroll
+        for (int j = 0; j < 8; j++) r[j] = (r[j] & ~keep) | (old[j] & keep);
+    }
+#pragma unroll
+    for (int j = 0; j < 8; j++) *reinterpret_cast<uint32_t *>(dst + 16 * j) = r[j];
 }
 
-// fp32 and fp16: grid-stride over the rows' VEC-wide pieces
-template <bool F16, int VEC>
+// fp32 and fp16: grid-stride over the rows' pieces of four
+template <bool F16>
 __global__ __launch_bounds__(WG) void k_kv_store(KvArgs a, int kvd) {
-    typedef float V __attribute__((ext_vector_type(VEC)));
     const int64_t p0 = a.pos ? (int64_t)*a.pos : a.pos0;
-    const int per = kvd / VEC;
+    const int per = kvd / 4;
     const int64_t n = (int64_t)a.n_tok * per;
     for (int64_t i = (int64_t)blockIdx.x * WG + threadIdx.x; i < n; i += (int64_t)gridDim.x * WG) {
         const int64_t b = i / per, t = p0 + b;
-        const int c = (int)(i % per) * VEC;
+        const int c = (int)(i % per) * 4;
         if (t < 0 || t >= a.ctx) continue;
-        const V x = *reinterpret_cast<const V *>(a.k + b * a.k_stride + c), y = *reinterpret_cast<const V *>(a.v + b * a.v_stride + c);
+        const f32x4 x = *reinterpret_cast<const RowV *>(a.k + b * a.k_stride + c), y = *reinterpret_cast<const RowV *>(a.v + b * a.v_stride + c);
         if (F16) {
-            typedef _Float16 H __attribute__((ext_vector_type(VEC)));
+            typedef _Float16 H __attribute__((ext_vector_type(4)));
             *reinterpret_cast<H *>(reinterpret_cast<_Float16 *>(a.kc) + t * kvd + c) = __builtin_convertvector(x, H);
             *reinterpret_cast<H *>(reinterpret_cast<_Float16 *>(a.vc) + t * kvd + c) = __builtin_convertvector(y, H);
         } else {
-            *reinterpret_cast<V *>(reinterpret_cast<float *>(a.kc) + t * kvd + c) = x;
-            *reinterpret_cast<V *>(reinterpret_cast<float *>(a.vc) + t * kvd + c) = y;
+            *reinterpret_cast<f32x4 *>(reinterpret_cast<float *>(a.kc) + t * kvd + c) = x;
+            *reinterpret_cast<f32x4 *>(reinterpret_cast<float *>(a.vc) + t * kvd + c) = y;
         }
     }
 }
@@ -163,43 +193,48 @@ __global__ __launch_bounds__(WG) void k_kv4_load(KvArgs a) {
             if (t < a.pos0 || t >= end) continue;
             const uint32_t w = *reinterpret_cast<const uint32_t *>(ct + kv_code_at(g * 16 + l, half * NB + b));
             const float d = h2f(*reinterpret_cast<const uint16_t *>(ct + kv_scale_at(HD, l / 4, b, l % 4, half)));
-            float *dst = out + (t - a.pos0) * a.k_stride + 8 * c;
+            RowV *dst = reinterpret_cast<RowV *>(out + (t - a.pos0) * a.k_stride + 8 * c);
 #pragma unroll
-            for (int j = 0; j < 8; j++) dst[j] = (float)((int)(w >> (4 * j) & 15) - 8) * d;
+            for (int h = 0; h < 2; h++) {
+                RowV x;
+#pragma unroll
+                for (int j = 0; j < 4; j++) x[j] = (float)((int)(w >> (16 * h + 4 * j) & 15) - 8) * d;
+                dst[h] = x;
+            }
         }
     } else {
-#pragma unroll 1
+#pragma unroll
         for (int u = 0; u < 4 * HD / WG; u++) {
             const int j = tid + u * WG, dim = j % HD, g = j / HD, b = dim / QB;
             const uint32_t w = *reinterpret_cast<const uint32_t *>(ct + kv_code_at(g * 16 + dim % 16, dim / 16));
+            const i32x4 ds = *reinterpret_cast<const i32x4 *>(ct + kv_scale_at(HD, g, b, 0, 0));   // [i][s]
 #pragma unroll
             for (int n = 0; n < 8; n++) {
                 const int64_t t = t0 + 16 * (n / 4) + 4 * g + n % 4;
                 if (t < a.pos0 || t >= end) continue;
-                const float d = h2f(*reinterpret_cast<const uint16_t *>(ct + kv_scale_at(HD, g, b, n % 4, n / 4)));
+                const float d = h2f((uint16_t)(ds[n % 4] >> (16 * (n / 4))));
                 out[(t - a.pos0) * a.k_stride + dim] = (float)((int)(w >> (4 * n) & 15) - 8) * d;
             }
         }
     }
 }
 
-template <bool F16, int VEC>
+template <bool F16>
 __global__ __launch_bounds__(WG) void k_kv_load(KvArgs a, int kvd) {
-    typedef float V __attribute__((ext_vector_type(VEC)));
-    const int per = kvd / VEC;
+    const int per = kvd / 4;
     const int64_t n = (int64_t)a.n_tok * per;
     const uint8_t *src = a.which ? a.vc : a.kc;
     for (int64_t i = (int64_t)blockIdx.x * WG + threadIdx.x; i < n; i += (int64_t)gridDim.x * WG) {
         const int64_t b = i / per, t = a.pos0 + b;
-        const int c = (int)(i % per) * VEC;
-        V x;
+        const int c = (int)(i % per) * 4;
+        f32x4 x;
         if (F16) {
-            typedef _Float16 H __attribute__((ext_vector_type(VEC)));
-            x = __builtin_convertvector(*reinterpret_cast<const H *>(reinterpret_cast<const _Float16 *>(src) + t * kvd + c), V);
+            typedef _Float16 H __attribute__((ext_vector_type(4)));
+            x = __builtin_convertvector(*reinterpret_cast<const H *>(reinterpret_cast<const _Float16 *>(src) + t * kvd + c), f32x4);
         } else {
-            x = *reinterpret_cast<const V *>(reinterpret_cast<const float *>(src) + t * kvd + c);
+            x = *reinterpret_cast<const f32x4 *>(reinterpret_cast<const float *>(src) + t * kvd + c);
         }
-        *reinterpret_cast<V *>(a.out + b * a.k_stride + c) = x;
+        *reinterpret_cast<RowV *>(a.out + b * a.k_stride + c) = x;
     }
 }
 
@@ -247,16 +282,9 @@ int launch_cache_store(hipStream_t st, const EhipCache &c, const EhipCacheRows &
         if (c.head_dim == 128) hipLaunchKernelGGL(k_kv4_store<128>, grid, dim3(WG), 0, st, a);
         else hipLaunchKernelGGL(k_kv4_store<64>, grid, dim3(WG), 0, st, a);
     } else {
-        // 16-byte loads where every row and piece is aligned for them
-        const bool vec = r.k_stride % 4 == 0 && r.v_stride % 4 == 0 && aligned(r.k, 16) && aligned(r.v, 16);
-        const dim3 grid = row_grid((int64_t)r.n_tok * kvd / (vec ? 4 : 1));
-        if (c.type == EHIP_KV_F16) {
-            if (vec) hipLaunchKernelGGL((k_kv_store<true, 4>), grid, dim3(WG), 0, st, a, kvd);
-            else hipLaunchKernelGGL((k_kv_store<true, 1>), grid, dim3(WG), 0, st, a, kvd);
-        } else {
-            if (vec) hipLaunchKernelGGL((k_kv_store<false, 4>), grid, dim3(WG), 0, st, a, kvd);
-            else hipLaunchKernelGGL((k_kv_store<false, 1>), grid, dim3(WG), 0, st, a, kvd);
-        }
+        const dim3 grid = row_grid((int64_t)r.n_tok * kvd / 4);
+        if (c.type == EHIP_KV_F16) hipLaunchKernelGGL(k_kv_store<true>, grid, dim3(WG), 0, st, a, kvd);
+        else hipLaunchKernelGGL(k_kv_store<false>, grid, dim3(WG), 0, st, a, kvd);
     }
     return hipGetLastError() == hipSuccess ? 0 : -1;
 }
@@ -306,15 +334,9 @@ extern "C" int ehip_cache_load(const EhipCache *c, int which, int64_t pos0, int 
         if (c->head_dim == 128) hipLaunchKernelGGL(k_kv4_load<128>, grid, dim3(WG), 0, st, a);
         else hipLaunchKernelGGL(k_kv4_load<64>, grid, dim3(WG), 0, st, a);
     } else {
-        const bool vec = out_stride % 4 == 0 && aligned(out, 16);
-        const dim3 grid = row_grid((int64_t)n_pos * kvd / (vec ? 4 : 1));
-        if (c->type == EHIP_KV_F16) {
-            if (vec) hipLaunchKernelGGL((k_kv_load<true, 4>), grid, dim3(WG), 0, st, a, kvd);
-            else hipLaunchKernelGGL((k_kv_load<true, 1>), grid, dim3(WG), 0, st, a, kvd);
-        } else {
-            if (vec) hipLaunchKernelGGL((k_kv_load<false, 4>), grid, dim3(WG), 0, st, a, kvd);
-            else hipLaunchKernelGGL((k_kv_load<false, 1>), grid, dim3(WG), 0, st, a, kvd);
-        }
+        const dim3 grid = row_grid((int64_t)n_pos * kvd / 4);
+        if (c->type == EHIP_KV_F16) hipLaunchKernelGGL(k_kv_load<true>, grid, dim3(WG), 0, st, a, kvd);
+        else hipLaunchKernelGGL(k_kv_load<false>, grid, dim3(WG), 0, st, a, kvd);
     }
     if (hipGetLastError() != hipSuccess) return refuse("%s: launch failed", who);
     return 0;
