@@ -11,6 +11,22 @@ typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
 typedef float f32x2 __attribute__((ext_vector_type(2)));
 typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
 
+// x / d for 0 <= x < 2^31, as x * m >> shift with m = ceil(2^(31 + l) / d), l =
+// ceil(log2 d): m d exceeds 2^(31 + l) by less than d <= 2^l, so x of that less
+// than 1 / d.  (A division by a number that is not constant takes 25
+// instructions, and a short launch is mostly its first and last microseconds.)
+struct Div {
+    uint32_t d, m, shift;
+    void set(uint32_t by) {
+        uint32_t l = 0;
+        while ((1ull << l) < by) l++;
+        d = by;
+        shift = 31 + l;
+        m = (uint32_t)(((1ull << shift) + by - 1) / by);
+    }
+    __device__ __forceinline__ int operator()(int x) const { return (int)((uint64_t)(uint32_t)x * m >> shift); }
+};
+
 struct AttendArgs {
     const float *q;
     float *out;
@@ -18,13 +34,13 @@ struct AttendArgs {
     const uint8_t *kc, *vc;
     int64_t head_bytes;          // 4 bits: bytes of a key head's tiles
     int kvd;                     // others: elements of a position
-    int n_tok, n_kv, G, pos0, ctx;
+    int n_tok, groups, pos0, ctx; // groups: of rows
+    Div n_kv, G, nsplit;          // key heads; query heads of each; workgroups that share a row group's positions
     const int *pos;
     int out_vec;                 // out rows take 16-byte stores
     int window, sinks;
     float qscale;                // scale * log2(e)
     int run;                     // tiles of a range (0: a unit's tiles over nsplit)
-    int nsplit;                  // workgroups that share a row group's positions
     float *part;                 // [unit][nsplit][rows][HD], then float4 [unit][nsplit][rows]; unit = (row group, key head)
     float4 *part_ml;             // a row's maximum, sum and score scale
     int *count;                  // [unit]: workgroups of the unit that are done; zero between launches
@@ -247,11 +263,11 @@ __device__ __forceinline__ void split_p(const f32x4 (&p)[2], float even, float o
 // dims d .. d + 3 of row r of key head kv: o / l
 template <int HD>
 __device__ __forceinline__ void store_out(const AttendArgs &a, int pos0, int kv, int r, int d, f32x4 o, float l) {
-    const int b = r / a.G;
+    const int b = a.G(r);
     const float inv = 1.0f / l;
     o *= inv;
     if (pos0 + b < 0 || pos0 + b >= a.ctx) o = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
-    float *dst = a.out + (int64_t)b * a.out_stride + (kv * a.G + r % a.G) * HD + d;
+    float *dst = a.out + (int64_t)b * a.out_stride + ((kv - b) * a.G.d + r) * HD + d;
     if (a.out_vec) {
         *reinterpret_cast<f32x4 *>(dst) = o;
     } else {
@@ -303,59 +319,80 @@ __device__ __forceinline__ void join_runs(const AttendArgs &a, int unit, int nac
     __syncthreads();
     if (!*last) return;
     if (tid == 0) __hip_atomic_store(a.count + unit, 0, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-    const Parts<HD, BR> P(a, (int64_t)unit * a.nsplit, nact);
-    const int nr = r1 - r0;
-    for (int r = wave; r < nr; r += NT / 64) {      // a wave a row, a lane a run: one round trip
-        const f32x4 ml = P.ml.get((min(lane, nact - 1) * BR + r) * 16);
-        const float m = lane < nact ? ml[0] : -INFINITY, M = wave_max(m);
-        const float f = m == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f((m - M) * ml[2]);
-        const float l = wave_sum(lane < nact ? f * ml[1] : 0.0f);
-        sf[r * AT_SPLITS + lane] = f;
-        if (lane == 0) sl[r] = l;
+    const Parts<HD, BR> P(a, (int64_t)unit * a.nsplit.d, nact);
+    // an item is four dims of a row.  A thread has U of them for Z runs at a time;
+    // where there are fewer items than threads, one for Z U runs, and `parts`
+    // threads share an item's runs.  The first loads are on their way before the
+    // weights are known (a round trip past the L2 is some 1.5 us).
+    constexpr int all = (BR * HD / 4 + NT - 1) / NT, U = all < 8 ? all : 8, Z = (BR == 32 && HD == 128 ? 24 : 16) / U;
+    const int nr = r1 - r0, items = nr * (HD / 4), parts = items <= NT / 2 ? NT / items : 1;
+    const int part = parts > 1 ? tid / items : 0, item = parts > 1 ? tid % items : tid;
+    f32x4 x[Z][U];
+    auto fetch = [&](int z0, int i0) {   // (z0: the same in all threads)
+#pragma unroll
+        for (int j = 0; j < Z; j++)
+#pragma unroll
+            for (int u = 0; u < U; u++) {
+                if (z0 + (parts > 1 ? (j * U + u) * parts : j) >= nact) continue;
+                const int z = parts > 1 ? z0 + (j * U + u) * parts + part : z0 + j, i = parts > 1 ? item : min(i0 + u * NT, items - 1);
+                x[j][u] = P.rows.get((min(z, nact - 1) * BR * (HD / 4) + i) * 16);
+            }
+    };
+    // a wave a row, a lane a run
+    constexpr int NW = NT / 64, RW = (BR + NW - 1) / NW < 8 ? (BR + NW - 1) / NW : 8;
+    f32x4 ml[RW];
+    auto fetch_ml = [&](int r) {
+#pragma unroll
+        for (int k = 0; k < RW; k++) ml[k] = P.ml.get((min(lane, nact - 1) * BR + min(r + k * NW, nr - 1)) * 16);
+    };
+    fetch_ml(wave);
+    fetch(0, item);
+    for (int r = wave; r < nr; r += RW * NW) {
+        if (r != wave) fetch_ml(r);
+#pragma unroll
+        for (int k = 0; k < RW; k++) {
+            const float m = lane < nact ? ml[k][0] : -INFINITY, M = wave_max(m);
+            const float f = m == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f((m - M) * ml[k][2]);
+            const float l = wave_sum(lane < nact ? f * ml[k][1] : 0.0f);
+            if (r + k * NW >= nr) break;
+            sf[(r + k * NW) * AT_SPLITS + lane] = f;
+            if (lane == 0) sl[r + k * NW] = l;
+        }
     }
     __syncthreads();
-    // an item is four dims of a row; 16 loads of a thread in flight
-    const int items = nr * (HD / 4), parts = NT / items;
-    if (parts > 1) {   // fewer items than threads: they share the runs
-        const int part = tid / items, i = tid % items, r = i / (HD / 4), d = i % (HD / 4) * 4;
+    if (parts > 1) {
+        const int r = item / (HD / 4);
         f32x4 o = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
-        if (part < parts) {
-            for (int z = part; z < nact; z += 16 * parts) {
-                f32x4 x[16];
+        for (int z0 = 0; z0 < nact; z0 += Z * U * parts) {
+            if (z0) fetch(z0, item);
 #pragma unroll
-                for (int j = 0; j < 16; j++) x[j] = P.rows.get(((min(z + j * parts, nact - 1) * BR + r) * HD + d) * 4);
-#pragma unroll
-                for (int j = 0; j < 16; j++) o += x[j] * (z + j * parts < nact ? sf[r * AT_SPLITS + z + j * parts] : 0.0f);
+            for (int j = 0; j < Z * U; j++) {
+                if (z0 + j * parts >= nact) continue;
+                const int z = z0 + j * parts + part;
+                const float f = sf[r * AT_SPLITS + min(z, nact - 1)];
+                o += x[j / U][j % U] * (part < parts && z < nact ? f : 0.0f);
             }
         }
         red[tid] = o;
         __syncthreads();
         if (tid >= items) return;
+#pragma unroll 8
         for (int q = 1; q < parts; q++) o += red[q * items + tid];
-        store_out<HD>(a, pos0, kv, r0 + r, d, o, sl[r]);
+        store_out<HD>(a, pos0, kv, r0 + r, item % (HD / 4) * 4, o, sl[r]);
         return;
     }
-    constexpr int all = (BR * HD / 4 + NT - 1) / NT, U = all < 8 ? all : 8;   // items of a thread at a time
     for (int i0 = tid; i0 < items; i0 += U * NT) {
         f32x4 o[U];
 #pragma unroll
         for (int u = 0; u < U; u++) o[u] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
-        for (int z = 0; z < nact; z += 2) {
-            f32x4 x[2][U];
+        for (int z = 0; z < nact; z += Z) {
+            if (z || i0 != tid) fetch(z, i0);
 #pragma unroll
-            for (int j = 0; j < 2; j++)
+            for (int j = 0; j < Z; j++) {
+                if (z + j >= nact) continue;
 #pragma unroll
-                for (int u = 0; u < U; u++) {
-                    const int i = min(i0 + u * NT, items - 1);
-                    x[j][u] = P.rows.get((min(z + j, nact - 1) * BR * (HD / 4) + i) * 16);
-                }
-#pragma unroll
-            for (int j = 0; j < 2; j++)
-#pragma unroll
-                for (int u = 0; u < U; u++) {
-                    const int r = min(i0 + u * NT, items - 1) / (HD / 4);
-                    o[u] += x[j][u] * (z + j < nact ? sf[r * AT_SPLITS + z + j] : 0.0f);
-                }
+                for (int u = 0; u < U; u++) o[u] += x[j][u] * sf[min(i0 + u * NT, items - 1) / (HD / 4) * AT_SPLITS + z + j];
+            }
         }
 #pragma unroll
         for (int u = 0; u < U; u++) {
@@ -367,6 +404,6 @@ __device__ __forceinline__ void join_runs(const AttendArgs &a, int unit, int nac
 
 // attend_rows.hip: units of ATTEND_ROWS rows
 constexpr int ATTEND_ROWS = 128;
-void launch_attend_rows(hipStream_t st, int hd, int64_t workgroups, const AttendArgs &a);
+void launch_attend_rows(hipStream_t st, int hd, dim3 grid, const AttendArgs &a);
 
 }  // namespace ehip

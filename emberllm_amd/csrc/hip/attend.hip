@@ -212,7 +212,7 @@ __device__ __forceinline__ void odd_values(const AttendArgs &a, Rows<HD, CT> &R,
                     for (int d = 0; d < HD / 16; d++)
 #pragma unroll
                         for (int r = 0; r < 4; r++) {
-                            const int64_t e = at + 16 * d + 4 * g + r;
+                            const int64_t e = at + HD / 16 * (4 * g + r) + d;
                             const float v = F16 ? (float)reinterpret_cast<const _Float16 *>(a.vc)[e] : reinterpret_cast<const float *>(a.vc)[e];
                             if (in && !(fabsf(v) < INFINITY)) R.o[c][d][r] += p * v;   // (not finite: 2^E does not matter)
                         }
@@ -220,13 +220,17 @@ __device__ __forceinline__ void odd_values(const AttendArgs &a, Rows<HD, CT> &R,
             }
 }
 
-// fp16: the lanes' pieces of K are 16-byte loads; a V operand is gathered from
-// 8 positions (64 bytes of a position to 16 lanes).  Positions past last_pos
-// repeat it.
+// fp16: the lanes' pieces of K and V are 16-byte loads (HD 128): lane l holds the
+// dims HD/16 l .. of its quarter's 8 positions, so that the d-th of each make
+// the V operand of the dims d, HD/16 + d, ... (one byte permutation a dword;
+// gathering 16 dims of a position by 2-byte loads took 205 us where this takes
+// 192, 16 heads of 128 and 4096 tokens).  Positions past last_pos repeat it.
 template <int HD, int CT, bool PACK, bool QL> struct Tile<EHIP_KV_F16, HD, CT, PACK, QL> {
     static constexpr int NB = (HD + 31) / 32;
     static constexpr int NH = PACK ? 1 : 2, QN = NB * NH;
-    i32x4 k[2][NB], v[HD / 16];
+    static constexpr int ND = HD / 16, NW2 = (ND + 1) / 2;   // dims of a lane, and their dwords
+    i32x4 k[2][NB];
+    int v[2][4][NW2];
     i32x4 Q[QL ? 1 : CT][QN];
     const i32x4 *ql;
     const _Float16 *kb, *vb;
@@ -264,14 +268,33 @@ template <int HD, int CT, bool PACK, bool QL> struct Tile<EHIP_KV_F16, HD, CT, P
     }
     __device__ __forceinline__ void load_v(const AttendArgs &a, int tile, int last_pos) {
         const int lane = threadIdx.x & 63, g = lane >> 4;
-        const uint16_t *base = reinterpret_cast<const uint16_t *>(vb) + (lane & 15);
 #pragma unroll
-        for (int i = 0; i < 4; i++) {
-            const int t = tile * KV_TILE + 4 * g + i;
-            const uint16_t *r0 = base + (int64_t)min(t, last_pos) * a.kvd, *r1 = base + (int64_t)min(t + 16, last_pos) * a.kvd;
+        for (int s = 0; s < 2; s++)
 #pragma unroll
-            for (int d = 0; d < HD / 16; d++) v[d][i] = (int)((uint32_t)r0[16 * d] | ((uint32_t)r1[16 * d] << 16));
-        }
+            for (int i = 0; i < 4; i++) {
+                const _Float16 *r = vb + (int64_t)min(tile * KV_TILE + 16 * s + 4 * g + i, last_pos) * a.kvd + ND * (lane & 15);
+                if constexpr (ND == 8) {
+                    const i32x4 x = *reinterpret_cast<const i32x4 *>(r);
+#pragma unroll
+                    for (int n = 0; n < 4; n++) v[s][i][n] = x[n];
+                } else if constexpr (ND == 4) {
+                    const int2 x = *reinterpret_cast<const int2 *>(r);
+                    v[s][i][0] = x.x;
+                    v[s][i][1] = x.y;
+                } else {
+                    static_assert(ND == 3, "three dims: 2-byte aligned");
+                    typedef int Int2 __attribute__((aligned(2)));
+                    v[s][i][0] = *reinterpret_cast<const Int2 *>(r);
+                    v[s][i][1] = reinterpret_cast<const uint16_t *>(r)[2];
+                }
+            }
+    }
+    // the V operand of the dims d, ND + d, ...: dword i holds d of positions 4g + i and 16 + 4g + i
+    __device__ __forceinline__ i32x4 v_at(int d) const {
+        i32x4 x;
+#pragma unroll
+        for (int i = 0; i < 4; i++) x[i] = (int)__builtin_amdgcn_perm((uint32_t)v[1][i][d / 2], (uint32_t)v[0][i][d / 2], d & 1 ? 0x07060302 : 0x05040100);
+        return x;
     }
     __device__ __forceinline__ void scores(f32x4 (&S)[CT][2]) {
 #pragma unroll
@@ -291,24 +314,28 @@ template <int HD, int CT, bool PACK, bool QL> struct Tile<EHIP_KV_F16, HD, CT, P
         bool odd = false;
         if (MASKED) {   // what is not finite goes to its own rows only
 #pragma unroll
-            for (int d = 0; d < HD / 16; d++)
+            for (int s = 0; s < 2; s++)
 #pragma unroll
-                for (int i = 0; i < 4; i++) {
-                    const bool a0 = (v[d][i] & 0x7c00) == 0x7c00, a1 = (v[d][i] & 0x7c000000) == 0x7c000000;
-                    odd |= a0 | a1;
-                    if (a0) v[d][i] &= (int)0xffff0000;
-                    if (a1) v[d][i] &= 0x0000ffff;
-                }
+                for (int i = 0; i < 4; i++)
+#pragma unroll
+                    for (int n = 0; n < NW2; n++) {
+                        int &w = v[s][i][n];
+                        const bool a0 = (w & 0x7c00) == 0x7c00, a1 = (w & 0x7c000000) == 0x7c000000;
+                        odd |= a0 | a1;
+                        w &= (a0 ? 0 : 0xffff) | (a1 ? 0 : (int)0xffff0000);
+                    }
         }
         softmax_step(R, S);
+        i32x4 hi[CT], lo[CT];
 #pragma unroll
-        for (int c = 0; c < CT; c++) {
-            i32x4 hi, lo;
-            split_p<PACK>(S[c], 0x1p14f, 0x1p14f, hi, lo);
+        for (int c = 0; c < CT; c++) split_p<PACK>(S[c], 0x1p14f, 0x1p14f, hi[c], lo[c]);
 #pragma unroll
-            for (int d = 0; d < HD / 16; d++) {
-                R.o[c][d] = mfma16(v[d], hi, R.o[c][d]);
-                if (!PACK) R.o[c][d] = mfma16(v[d], lo, R.o[c][d]);
+        for (int d = 0; d < ND; d++) {
+            const i32x4 x = v_at(d);
+#pragma unroll
+            for (int c = 0; c < CT; c++) {
+                if (!PACK) R.o[c][d] = mfma16(x, lo[c], R.o[c][d]);
+                R.o[c][d] = mfma16(x, hi[c], R.o[c][d]);
             }
         }
         if (MASKED && __any(odd)) odd_values<HD, CT, true, PACK>(a, R, S, t0, kv, last_pos);
@@ -318,7 +345,7 @@ template <int HD, int CT, bool PACK, bool QL> struct Tile<EHIP_KV_F16, HD, CT, P
 
 // fp32, on the fp32 matrix cores (16x16x4): lane quarter g supplies dims
 // g HD / 4 .. of K and Q, so its pieces are contiguous; a P.V step contracts
-// one position per quarter.
+// one position per quarter.  Lane l holds the dims HD/16 l .. of V, as for fp16.
 template <int HD, int CT, bool PACK, bool QL> struct Tile<EHIP_KV_F32, HD, CT, PACK, QL> {
     static_assert(!PACK, "fp32 rows have no low halves");
     static constexpr int NQ = HD / 16;   // 16-byte pieces of a quarter
@@ -362,9 +389,9 @@ template <int HD, int CT, bool PACK, bool QL> struct Tile<EHIP_KV_F32, HD, CT, P
         for (int s = 0; s < 2; s++)
 #pragma unroll
             for (int i = 0; i < 4; i++) {
-                const float *r = vb + (int64_t)min(tile * KV_TILE + 16 * s + 4 * g + i, last_pos) * a.kvd + (lane & 15);
+                const float *r = vb + (int64_t)min(tile * KV_TILE + 16 * s + 4 * g + i, last_pos) * a.kvd + HD / 16 * (lane & 15);
 #pragma unroll
-                for (int d = 0; d < HD / 16; d++) v[d][s][i] = r[16 * d];
+                for (int d = 0; d < HD / 16; d++) v[d][s][i] = r[d];
             }
     }
     __device__ __forceinline__ void scores(f32x4 (&S)[CT][2]) {
@@ -432,17 +459,15 @@ __device__ __forceinline__ void attend_body(const AttendArgs &a) {
     __shared__ float sm[NW][BR], sl[NW][BR], ssc[BR], se[NW];
     static_assert(join_floats(BR, 64 * NW) * 4 <= sizeof(so), "the join fits the waves' outputs");
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, g = lane >> 4;
-    const int nunits = gridDim.x / a.nsplit;
-    const int unit = blockIdx.x % nunits, split = blockIdx.x / nunits;
-    const int kv = unit % a.n_kv, groups = nunits / a.n_kv;
-    const int nrows = a.n_tok * a.G, r0 = (groups - 1 - unit / a.n_kv) * BR, r1 = min(r0 + BR, nrows);
+    const int unit = blockIdx.x, split = blockIdx.y, group = a.n_kv(unit), kv = unit - group * a.n_kv.d;
+    const int nrows = a.n_tok * a.G.d, r0 = (a.groups - 1 - group) * BR, r1 = min(r0 + BR, nrows);
     const int pos0 = a.pos ? max(min(*a.pos, a.ctx), -a.n_tok) : a.pos0;
     // rows whose position lies outside the cache (a device position only) give zeros
-    const int first_pos = max(pos0 + r0 / a.G, 0), last_pos = min(pos0 + (r1 - 1) / a.G, a.ctx - 1);
+    const int first_pos = max(pos0 + a.G(r0), 0), last_pos = min(pos0 + a.G(r1 - 1), a.ctx - 1);
     const Tiles T = tiles_seen(first_pos, last_pos, a.window, a.sinks);
     const int ntiles = last_pos < first_pos ? 0 : T.n;
-    const int run = max((ntiles + a.nsplit - 1) / a.nsplit, 1), nact = max((ntiles + run - 1) / run, 1);
-    if (split >= nact) return;
+    const int run = max(a.nsplit(ntiles + a.nsplit.d - 1), 1);
+    if (split && split * run >= ntiles) return;
     const int v1 = min((split + 1) * run, ntiles);
 
     Rows<HD, CT> R;
@@ -459,14 +484,14 @@ __device__ __forceinline__ void attend_body(const AttendArgs &a) {
     }
 #pragma unroll
     for (int c = 0; c < CT; c++) {
-        const int r = min(r0 + 16 * c + (lane & (PACK ? 7 : 15)), nrows - 1), b = r / a.G;
+        const int r = min(r0 + 16 * c + (lane & (PACK ? 7 : 15)), nrows - 1), b = a.G(r);
         R.p[c] = pos0 + b;
         R.m[c] = -INFINITY;
         R.l[c] = 0.0f;
 #pragma unroll
         for (int d = 0; d < HD / 16; d++) R.o[c][d] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
         if (QL && wave != c) continue;
-        X.load_q(a, a.q + (int64_t)b * a.q_stride + (kv * a.G + r % a.G) * HD, c, R.sc[c], ql);
+        X.load_q(a, a.q + (int64_t)b * a.q_stride + ((kv - b) * a.G.d + r) * HD, c, R.sc[c], ql);
         if (QL && g == 0) ssc[16 * c + lane] = R.sc[c];
     }
     if (QL) {
@@ -475,7 +500,7 @@ __device__ __forceinline__ void attend_body(const AttendArgs &a) {
         for (int c = 0; c < CT; c++) R.sc[c] = ssc[16 * c + (lane & 15)];
     }
     // positions that every row sees: up to that of the first row, and from the last row's window on (or a sink)
-    const int all_to = pos0 + r0 / a.G, all_from = a.window > 0 ? pos0 + (r1 - 1) / a.G - a.window + 1 : 0;
+    const int all_to = pos0 + a.G(r0), all_from = a.window > 0 ? pos0 + a.G(r1 - 1) - a.window + 1 : 0;
     while (vi < v1) {
         if (QL) asm volatile("" ::: "memory");   // (Q stays in LDS: the compiler would keep it in registers over the loop)
         const int tile = T.at(vi), t0 = tile * KV_TILE;
@@ -509,15 +534,23 @@ __device__ __forceinline__ void attend_body(const AttendArgs &a) {
         for (int d = 0; d < HD / 16; d++) {
             f32x4 o = R.o[c][d];
             if (PACK) o = add_halves(o);
-            if (!(PACK && (lane & 8))) *reinterpret_cast<f32x4 *>(&so[wave][r][16 * d + 4 * g]) = o;
+            if (PACK && (lane & 8)) continue;
+            if (TYPE == EHIP_KV_Q4) {
+                *reinterpret_cast<f32x4 *>(&so[wave][r][16 * d + 4 * g]) = o;
+            } else {
+#pragma unroll
+                for (int i = 0; i < 4; i++) so[wave][r][HD / 16 * (4 * g + i) + d] = o[i];
+            }
         }
     }
     if (lane == 0) se[wave] = __builtin_amdgcn_ldexpf(1.0f, -E);
     __syncthreads();
-    const bool alone = nact == 1;
-    const Parts<HD, BR> mine(a, (int64_t)unit * a.nsplit + split, 1);
-    for (int i = tid; i < BR * (HD / 4); i += 64 * NW) {
-        const int r = i / (HD / 4), d = i % (HD / 4) * 4;
+    const bool alone = ntiles <= run;
+    const Parts<HD, BR> mine(a, (int64_t)unit * a.nsplit.d + split, 1);
+#pragma unroll
+    for (int i0 = 0; i0 < BR * (HD / 4); i0 += 64 * NW) {
+        const int i = i0 + tid, r = i / (HD / 4), d = i % (HD / 4) * 4;
+        if (BR * (HD / 4) % (64 * NW) && r >= BR) break;
         float M = sm[0][r];
 #pragma unroll
         for (int w = 1; w < NW; w++) M = fmaxf(M, sm[w][r]);
@@ -539,7 +572,7 @@ __device__ __forceinline__ void attend_body(const AttendArgs &a) {
     }
     if (alone) return;
 
-    join_runs<HD, BR, 64 * NW>(a, unit, nact, r0, r1, pos0, kv, &so[0][0][0]);
+    join_runs<HD, BR, 64 * NW>(a, unit, (ntiles + run - 1) / run, r0, r1, pos0, kv, &so[0][0][0]);
 }
 
 template <int TYPE, int HD, int CT, bool PACK, int NW>
@@ -564,6 +597,30 @@ constexpr int MAX_UNITS = 2 * SLOTS;   // units from which on none is split
 
 static int tiles_of_rows(int64_t pos0, int64_t r0, int64_t r1, int G, int window, int sinks) {
     return tiles_seen((int)(pos0 + r0 / G), (int)(pos0 + (r1 - 1) / G), window, sinks).n;
+}
+
+// Into how many ranges a unit's tiles are cut, each for a workgroup: the least
+// time, counted in fifths of what a wave takes for a tile by itself (7 beside a
+// second wave on its SIMD).  A workgroup's start and end take three tiles, a join
+// two (16 heads of 128 over 4 bits: a range of one tile per wave 8.5 us, of two
+// 10.6, of five 16.3, one tile and a join 12.9).  23 tokens at 517, 17 tiles of
+// 16 units: 5 ranges 13.4 us, one 16.3; a prompt of 700, up to 22 tiles of 352
+// units: one range 19.4, two 26.4; 300 tokens at 4000, 135 of 152: three 46.5,
+// four, which do not run at once, 54.6.
+// slots: workgroups that the GPU holds at a time.
+static int ranges(int64_t units, int tiles, int waves, int64_t slots) {
+    int64_t best = 0;
+    int n = 1;
+    for (int z = 1; z <= AT_SPLITS; z++) {
+        const int64_t wgs = units * z, k = ((tiles + z - 1) / z + waves - 1) / waves;
+        if (z > 1 && (wgs > 2 * slots || tiles <= (z - 1) * waves)) break;
+        const int64_t cost = (wgs + slots - 1) / slots * (15 + k * (2 * wgs > slots ? 7 : 5)) + (z > 1 ? 10 : 0);
+        if (z == 1 || cost < best) {
+            best = cost;
+            n = z;
+        }
+    }
+    return n;
 }
 
 static int few_rows(int type, int64_t rows) { return type != EHIP_KV_F32 && rows <= 8 ? 8 : rows <= 16 ? 16 : 32; }
@@ -601,9 +658,9 @@ static Shape shape_of(const EhipCache &c, const EhipAttend &q) {
     } else {
         tiles = tiles_of_rows(pos0, (groups - 1) * s.br, rows, G, q.window, q.sinks);
         if (c.type == EHIP_KV_Q4 && s.br <= 16 && s.units * ((tiles + 3) / 4) > 256) s.waves = 8;
-        // two waves to each SIMD, each with at least a tile
-        const int64_t most = (tiles + s.waves - 1) / s.waves, slots = SLOTS * 4 / s.waves, want = s.units >= slots ? 1 : (slots + s.units - 1) / s.units;
-        s.nsplit = (int)(want < most ? want : most);
+        // (32 rows of 128 dims over fp32 take more than half of a SIMD's registers)
+        const int simd_waves = c.type == EHIP_KV_F32 && c.head_dim == 128 && s.br == 32 ? 1 : 2;
+        s.nsplit = ranges(s.units, tiles, s.waves, SLOTS / 2 * simd_waves * 4 / s.waves);
     }
     if (s.nsplit > AT_SPLITS) {
         s.nsplit = AT_SPLITS;
@@ -621,7 +678,7 @@ static int64_t space_rows(const Shape &s) { return s.nsplit > 1 ? s.units * s.ns
 
 template <int TYPE, int HD>
 static int attend_go(hipStream_t st, const AttendArgs &a, const Shape &s) {
-    const dim3 grid((unsigned)(s.units * s.nsplit)), wg(64 * s.waves);
+    const dim3 grid((unsigned)s.units, (unsigned)s.nsplit), wg(64 * s.waves);
     if constexpr (TYPE != EHIP_KV_F32) {
         if (s.br == 8 && s.waves == 4) hipLaunchKernelGGL((k_attend<TYPE, HD, 1, true, 4>), grid, wg, 0, st, a);
     }
@@ -634,7 +691,7 @@ static int attend_go(hipStream_t st, const AttendArgs &a, const Shape &s) {
         if constexpr (q_in_lds(TYPE, HD, 2)) hipLaunchKernelGGL((k_attend_two<TYPE, HD, 2, false, 4>), grid, wg, 0, st, a);
         else hipLaunchKernelGGL((k_attend<TYPE, HD, 2, false, 4>), grid, wg, 0, st, a);
     }
-    if (TYPE == EHIP_KV_F32 && s.br == ATTEND_ROWS) launch_attend_rows(st, HD, s.units * s.nsplit, a);
+    if (TYPE == EHIP_KV_F32 && s.br == ATTEND_ROWS) launch_attend_rows(st, HD, grid, a);
     const hipError_t e = hipGetLastError();
     return e == hipSuccess ? 0 : refuse("ehip_attend: launch: %s", hipGetErrorString(e));
 }
@@ -657,10 +714,10 @@ int launch_attend(hipStream_t st, const EhipCache &c, const EhipAttend &q) {
     a.kc = static_cast<const uint8_t *>(c.k); a.vc = static_cast<const uint8_t *>(c.v);
     a.head_bytes = (c.ctx + KV_TILE - 1) / KV_TILE * kv_tile_bytes(c.head_dim);
     a.kvd = c.n_kv * c.head_dim;
-    a.n_tok = q.n_tok; a.n_kv = c.n_kv; a.G = q.n_heads / c.n_kv; a.pos0 = q.pos0; a.ctx = (int)c.ctx; a.pos = q.pos;
+    a.n_tok = q.n_tok; a.groups = (int)(s.units / c.n_kv); a.pos0 = q.pos0; a.ctx = (int)c.ctx; a.pos = q.pos;
     a.window = q.window; a.sinks = q.sinks;
     a.qscale = (q.scale != 0.0f ? q.scale : 1.0f / sqrtf((float)c.head_dim)) * 1.4426950408889634f;
-    a.nsplit = s.nsplit;
+    a.n_kv.set(c.n_kv); a.G.set(q.n_heads / c.n_kv); a.nsplit.set(s.nsplit);
     a.run = s.run;
     a.out_vec = aligned(q.out, 16) && q.out_stride % 4 == 0;
     if (s.nsplit > 1) {
@@ -700,13 +757,14 @@ extern "C" uint64_t ehip_attend_workspace(const EhipCache *c, int n_heads, int n
     uint64_t most = 0;
     // On the way to n_tok tokens a unit's rows go through at most four sizes;
     // the largest count of tokens of each, U units of it and T tiles at most.
-    // Few rows: at most SLOTS - 1 + U workgroups.  Many: tiles per unit grow
-    // along a prompt ever more slowly, so the average is at least half of the
-    // most, and with it a range: U (2 SLOTS / U + 1), and U more for rounding.
+    // Few rows: at most 2 SLOTS workgroups, of at least a tile to each of four
+    // waves.  Many: tiles per unit grow along a prompt ever more slowly, so the
+    // average is at least half of the most, and with it a range: U (2 SLOTS / U +
+    // 1), and U more for rounding.
     auto bound = [&](int64_t rows, int br) {
         const bool many = br == ATTEND_ROWS;
-        const int64_t units = (rows + br - 1) / br * c->n_kv, top = many ? MAX_UNITS - 1 : SLOTS - 1, U = units < top ? units : top;
-        const int64_t wgs = many ? 2 * SLOTS + 2 * U : SLOTS - 1 + U, by_tiles = U * ((tiles + (many ? 7 : 3)) / (many ? 8 : 4));
+        const int64_t units = (rows + br - 1) / br * c->n_kv, U = units < MAX_UNITS ? units : MAX_UNITS;
+        const int64_t wgs = many ? 2 * SLOTS + 2 * U : 2 * SLOTS, by_tiles = U * ((tiles + (many ? 7 : 3)) / (many ? 8 : 4));
         const uint64_t b = by_tiles > U ? space_bytes((wgs < by_tiles ? wgs : by_tiles) * br, c->head_dim) : 0;
         if (b > most) most = b;
     };

@@ -177,16 +177,14 @@ __global__ __launch_bounds__(64 * AR_NW, 2) void k_attend_rows(AttendArgs a) {
     __shared__ __align__(16) uint8_t lds[BYTES];
     S *buf = reinterpret_cast<S *>(lds);
     const int tid = threadIdx.x, lane = tid & 63, wave = wave_id(), g = lane >> 4, l = lane & 15;
-    const int nunits = gridDim.x / a.nsplit;
-    const int unit = blockIdx.x % nunits, split = blockIdx.x / nunits;
-    const int kv = unit % a.n_kv, groups = nunits / a.n_kv, k = unit / a.n_kv;
-    const int nrows = a.n_tok * a.G, r0 = (groups - 1 - k) * AR_BR, r1 = min(r0 + AR_BR, nrows);
+    const int unit = blockIdx.x, split = blockIdx.y, group = a.n_kv(unit), kv = unit - group * a.n_kv.d;
+    const int nrows = a.n_tok * a.G.d, r0 = (a.groups - 1 - group) * AR_BR, r1 = min(r0 + AR_BR, nrows);
     const int pos0 = a.pos ? max(min(*a.pos, a.ctx), -a.n_tok) : a.pos0;
-    const int first_pos = max(pos0 + r0 / a.G, 0), last_pos = min(pos0 + (r1 - 1) / a.G, a.ctx - 1);
+    const int first_pos = max(pos0 + a.G(r0), 0), last_pos = min(pos0 + a.G(r1 - 1), a.ctx - 1);
     const Tiles T = tiles_seen(first_pos, last_pos, a.window, a.sinks);
     const int ntiles = last_pos < first_pos ? 0 : T.n;
-    const int run = max(max((ntiles + a.nsplit - 1) / a.nsplit, a.run), 1), nact = max((ntiles + run - 1) / run, 1);
-    if (split >= nact) return;
+    const int run = max(max(a.nsplit(ntiles + a.nsplit.d - 1), a.run), 1);
+    if (split && split * run >= ntiles) return;
     const int v0 = split * run, v1 = min(v0 + run, ntiles);
 
     Stager<HD> X;
@@ -199,17 +197,17 @@ __global__ __launch_bounds__(64 * AR_NW, 2) void k_attend_rows(AttendArgs a) {
     QHalf<HD, false> Q[CT];
 #pragma unroll
     for (int c = 0; c < CT; c++) {
-        const int r = min(w0 + 16 * c + l, nrows - 1), b = r / a.G;
+        const int r = min(w0 + 16 * c + l, nrows - 1), b = a.G(r);
         R.p[c] = pos0 + b;
         R.m[c] = -INFINITY;
         R.l[c] = 0.0f;
 #pragma unroll
         for (int d = 0; d < ND; d++) R.o[c][d] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
-        load_q16<HD, false, false>(a, a.q + (int64_t)b * a.q_stride + (kv * a.G + r % a.G) * HD, Q[c], R.sc[c]);
+        load_q16<HD, false, false>(a, a.q + (int64_t)b * a.q_stride + ((kv - b) * a.G.d + r) * HD, Q[c], R.sc[c]);
     }
     // positions that all rows of the workgroup, and of the wave, see (or a sink's), and that any of the wave sees
-    const int all_to = pos0 + r0 / a.G, all_from = a.window > 0 ? pos0 + (r1 - 1) / a.G - a.window + 1 : 0;
-    const int mine_to = pos0 + w0 / a.G, mine_last = w0 < nrows ? pos0 + (w1 - 1) / a.G : -1;
+    const int all_to = pos0 + a.G(r0), all_from = a.window > 0 ? pos0 + a.G(r1 - 1) - a.window + 1 : 0;
+    const int mine_to = pos0 + a.G(w0), mine_last = w0 < nrows ? pos0 + a.G(w1 - 1) : -1;
     const int mine_from = a.window > 0 ? mine_last - a.window + 1 : 0, mine_first = a.window > 0 ? mine_to - a.window + 1 : 0;
     auto masked = [&](int t0) { return !(t0 + KV_TILE - 1 <= all_to && (t0 >= all_from || t0 + KV_TILE <= a.sinks)); };
     i32x4 vexp = { 0, 0, 0, 0 };   // the power of two of V that the output's sums carry, by staging wave's dims
@@ -293,8 +291,8 @@ __global__ __launch_bounds__(64 * AR_NW, 2) void k_attend_rows(AttendArgs a) {
         lds_barrier();
     }
 
-    const bool alone = nact == 1;
-    const Parts<HD, AR_BR> mine_parts(a, (int64_t)unit * a.nsplit + split, 1);
+    const bool alone = ntiles <= run;
+    const Parts<HD, AR_BR> mine_parts(a, (int64_t)unit * a.nsplit.d + split, 1);
 #pragma unroll
     for (int c = 0; c < CT; c++) {
         const float sum = quarters_sum(R.l[c]);
@@ -310,11 +308,11 @@ __global__ __launch_bounds__(64 * AR_NW, 2) void k_attend_rows(AttendArgs a) {
         }
         if (!alone && g == 0 && r < nrows) mine_parts.ml.put((r - r0) * 16, f32x4{R.m[c], sum, R.sc[c], 0.0f});
     }
-    if (!alone) join_runs<HD, AR_BR, 64 * AR_NW>(a, unit, nact, r0, r1, pos0, kv, reinterpret_cast<float *>(lds));
+    if (!alone) join_runs<HD, AR_BR, 64 * AR_NW>(a, unit, (ntiles + run - 1) / run, r0, r1, pos0, kv, reinterpret_cast<float *>(lds));
 }
 
-void launch_attend_rows(hipStream_t st, int hd, int64_t workgroups, const AttendArgs &a) {
-    const dim3 grid((unsigned)workgroups), wg(64 * AR_NW);
+void launch_attend_rows(hipStream_t st, int hd, dim3 grid, const AttendArgs &a) {
+    const dim3 wg(64 * AR_NW);
     if (hd == 48) hipLaunchKernelGGL((k_attend_rows<48>), grid, wg, 0, st, a);
     if (hd == 64) hipLaunchKernelGGL((k_attend_rows<64>), grid, wg, 0, st, a);
     if (hd == 128) hipLaunchKernelGGL((k_attend_rows<128>), grid, wg, 0, st, a);
