@@ -26,8 +26,8 @@
 // Codes are exact in fp16; a score is the sum over its blocks of (block's
 // product) * d in fp32.  A value (code - 8) d has at most 15 bits, so hi =
 // fp16((code - 8) d) and lo = (code - 8) d - hi hold it exactly at any fp16 d.
-// Probabilities are split times 2^14 (what a half loses at its smallest is
-// 2^-39 of the largest), which the outputs' sums carry until the end; of the
+// Probabilities, 4 at most, are split times 2^13 (what a half loses at its
+// smallest is 2^-38), which the outputs' sums carry until the end; of the
 // four products of halves the smallest, lo.lo below 2^-24 of the whole, is
 // left out where it is not free.  fp16 caches are one half already; an fp32
 // cache goes through the fp32 matrix cores as it is.
@@ -54,7 +54,7 @@ template <int HD, int CT, bool PACK, bool QL> struct Tile<EHIP_KV_Q4, HD, CT, PA
     i32x4 k[NP], v[NP], ks[NB], vs[NB];
     i32x4 Q[QL ? 1 : CT][QN];
     const i32x4 *ql;
-    int E = 14;                  // the outputs' sums carry 2^E: 14, or 6 once a value was 4096 and more
+    int E = 13;                  // the outputs' sums carry 2^E: 13, or 5 once a value was 4096 and more
     const uint8_t *kb, *vb;
     uint32_t magic;
 
@@ -155,16 +155,16 @@ template <int HD, int CT, bool PACK, bool QL> struct Tile<EHIP_KV_Q4, HD, CT, PA
                 }
         }
         const bool big = large();
-        softmax_step(R, S, big && E == 14 ? 0x1p-8f : 1.0f);
+        softmax_step(R, S, big && E == 13 ? 0x1p-8f : 1.0f);
         if (big) {
-            E = 6;
+            E = 5;
             const f16x2 down = { (_Float16)0x1p-8f, (_Float16)0x1p-8f };
 #pragma unroll
             for (int b = 0; b < NB; b++)
 #pragma unroll
                 for (int i = 0; i < 4; i++) vs[b][i] = dword(halves(vs[b][i]) * down);
         }
-        const float even = big || E == 14 ? 0x1p14f : 0x1p6f, odd = even * 0.0625f;   // (the codes of odd i are 16 times too large)
+        const float even = big || E == 13 ? 0x1p13f : 0x1p5f, odd = even * 0.0625f;   // (the codes of odd i are 16 times too large)
         i32x4 hi[CT], lo[CT];
 #pragma unroll
         for (int c = 0; c < CT; c++) split_p<PACK>(S[c], even, odd, hi[c], lo[c]);
@@ -328,7 +328,7 @@ template <int HD, int CT, bool PACK, bool QL> struct Tile<EHIP_KV_F16, HD, CT, P
         softmax_step(R, S);
         i32x4 hi[CT], lo[CT];
 #pragma unroll
-        for (int c = 0; c < CT; c++) split_p<PACK>(S[c], 0x1p14f, 0x1p14f, hi[c], lo[c]);
+        for (int c = 0; c < CT; c++) split_p<PACK>(S[c], 0x1p13f, 0x1p13f, hi[c], lo[c]);
 #pragma unroll
         for (int d = 0; d < ND; d++) {
             const i32x4 x = v_at(d);
@@ -340,7 +340,7 @@ template <int HD, int CT, bool PACK, bool QL> struct Tile<EHIP_KV_F16, HD, CT, P
         }
         if (MASKED && __any(odd)) odd_values<HD, CT, true, PACK>(a, R, S, t0, kv, last_pos);
     }
-    __device__ __forceinline__ int exponent() const { return 14; }
+    __device__ __forceinline__ int exponent() const { return 13; }
 };
 
 // fp32, on the fp32 matrix cores (16x16x4): lane quarter g supplies dims

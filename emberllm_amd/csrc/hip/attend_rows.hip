@@ -276,7 +276,7 @@ __global__ __launch_bounds__(64 * AR_NW, 2) void k_attend_rows(AttendArgs a) {
             softmax_step(R, P);
             i32x4 hi[CT], lo[CT];
 #pragma unroll
-            for (int c = 0; c < CT; c++) split_p<false>(P[c], 0x1p14f, 0x1p14f, hi[c], lo[c]);
+            for (int c = 0; c < CT; c++) split_p<false>(P[c], 0x1p13f, 0x1p13f, hi[c], lo[c]);
 #pragma unroll
             for (int d = 0; d < ND; d++) {
                 const i32x4 vh = t.v[0][d][lane], vl = t.v[1][d][lane];
@@ -301,7 +301,7 @@ __global__ __launch_bounds__(64 * AR_NW, 2) void k_attend_rows(AttendArgs a) {
         for (int d = 0; d < ND; d++) {
             f32x4 o;
 #pragma unroll
-            for (int i = 0; i < 4; i++) o[i] = __builtin_amdgcn_ldexpf(R.o[c][d][i], -14 - vexp[d / NV]);
+            for (int i = 0; i < 4; i++) o[i] = __builtin_amdgcn_ldexpf(R.o[c][d][i], -13 - vexp[d / NV]);
             if (r >= nrows) continue;
             if (alone) store_out<HD>(a, pos0, kv, r, 16 * d + 4 * g, o, sum);
             else mine_parts.rows.put(((r - r0) * HD + 16 * d + 4 * g) * 4, o);

@@ -207,10 +207,11 @@ def attended(q, k, v, pos0, window=0, sinks=0, scale=0.0):
     at most twice its weights' relative error times sum p |v|.
 
     fp16 halves also lose what lies below half their smallest step, 2^-25.  A
-    weight (4 bits: times its block's scale d) reaches them multiplied so that
-    the largest possible one is at least 2^14 (of the largest d), so each of
-    the N positions loses at most 2^-39 of 1 (of max d, and a code is at most
-    8 of it): 2^-39 N max |v|, before a division by a sum of at least 1."""
+    weight reaches them relative to a score within 2 (in powers of two) below
+    the row's largest so far, so it is 4 at most and goes in times 2^13 without
+    leaving fp16; each of the N positions loses at most 2^-25 2^-13 of 1:
+    2^-38 N max |v|, before a division by a sum of at least 1 (the largest
+    score's own weight is 1 or more)."""
     n, nh, hd = q.shape
     ctx, nkv = k.shape[:2]
     q, k, v = (t.astype(np.float64) for t in (q, k, v))
@@ -237,10 +238,10 @@ def attended(q, k, v, pos0, window=0, sinks=0, scale=0.0):
                 if h % (nh // nkv) == 0:
                     top = np.array([np.abs(vv[j]).max(initial=0) for j in seen])
                 out[:, h] = w @ vv
-                bound[:, h] = 2 * rel[:, None] * (w @ np.abs(vv)) + 2.0 ** -39 * (seen.sum(1) * top)[:, None] + 1e-38
+                bound[:, h] = 2 * rel[:, None] * (w @ np.abs(vv)) + 2.0 ** -38 * (seen.sum(1) * top)[:, None] + 1e-38
                 continue
             for i in range(n):
                 j = seen[i]
                 out[i, h] = w[i, j] @ vv[j]
-                bound[i, h] = 2 * rel[i] * (w[i, j] @ np.abs(vv[j])) + 2.0 ** -39 * j.sum() * np.abs(vv[j]).max(initial=0) + 1e-38
+                bound[i, h] = 2 * rel[i] * (w[i, j] @ np.abs(vv[j])) + 2.0 ** -38 * j.sum() * np.abs(vv[j]).max(initial=0) + 1e-38
     return out, bound
