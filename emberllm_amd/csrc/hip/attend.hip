@@ -699,6 +699,7 @@ static int attend_go(hipStream_t st, const AttendArgs &a, const Shape &s) {
 // How a call is shared over workgroups; -1 where its workspace does not do.
 static int shape_call(const EhipCache &c, const EhipAttend &q, Shape *s) {
     *s = shape_of(c, q);
+    if (s->units * 64 * s->waves > UINT32_MAX) return refuse("ehip_attend: %d tokens of %d heads are more than a launch's threads", q.n_tok, q.n_heads);
     const uint64_t need = space_bytes(space_rows(*s), c.head_dim);
     if (need && (!q.workspace || !aligned(q.workspace, 16) || q.workspace_bytes < need))
         return refuse("ehip_attend: the workspace is null, not 16-byte aligned, or smaller than this call's %llu bytes", (unsigned long long)need);

@@ -20,6 +20,8 @@
 #include <cstdio>
 #include <cstdlib>
 #include <cstring>
+#include <memory>
+#include <new>
 #include <vector>
 
 #include "../../../include/ember.h"
@@ -1573,10 +1575,11 @@ static int kv_copy(EhipState *s, int which, int layer, int n_pos, void *host, bo
     const size_t row = (size_t)c.n_kv_heads * c.head_dim * s->esize, layer_bytes = s->opt ? s->layer_bytes : (size_t)s->ctx * row;
     uint8_t *base = static_cast<uint8_t *>(which ? s->vc : s->kc) + (size_t)layer * layer_bytes;
     if (s->opt && s->kv_type == EHIP_KV_Q4) {
-        std::vector<uint8_t> tiles(layer_bytes);
-        HCHK(hipMemcpy(tiles.data(), base, layer_bytes, hipMemcpyDeviceToHost), -1);
-        q4_rows(c, tiles.data(), (s->ctx + KV_TILE - 1) / KV_TILE, which != 0, n_pos, static_cast<uint8_t *>(host), write);
-        if (write) HCHK(hipMemcpy(base, tiles.data(), layer_bytes, hipMemcpyHostToDevice), -1);
+        const std::unique_ptr<uint8_t[]> tiles(new (std::nothrow) uint8_t[layer_bytes]);
+        if (!tiles) { set_err("kv_%s: %zu bytes of host memory", write ? "write" : "read", layer_bytes); return -1; }
+        HCHK(hipMemcpy(tiles.get(), base, layer_bytes, hipMemcpyDeviceToHost), -1);
+        q4_rows(c, tiles.get(), (s->ctx + KV_TILE - 1) / KV_TILE, which != 0, n_pos, static_cast<uint8_t *>(host), write);
+        if (write) HCHK(hipMemcpy(base, tiles.get(), layer_bytes, hipMemcpyHostToDevice), -1);
         return 0;
     }
     if (write) HCHK(hipMemcpy(base, host, row * n_pos, hipMemcpyHostToDevice), -1);

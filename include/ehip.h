@@ -235,7 +235,7 @@ int ehip_cache_load(const EhipCache *cache, int which, int64_t pos0, int n_pos, 
  * Query head h of a token uses key head h / (n_heads / n_kv).  out rows:
  * softmax(q.k * scale) v.  What a token does not see does not reach its rows,
  * whatever the cache holds there; a row that sees keys or values that are not
- * finite need not be finite. */
+ * finite need not be finite.  out does not overlap q. */
 typedef struct {
     const float   *q;
     float         *out;

@@ -130,6 +130,13 @@ def test_attend_refuses():
         refused(L.ehip_attend(big, call(pos0=4000, **kw), None), "workspace")
 
 
+def test_attend_refuses_what_no_launch_holds():
+    c = cache(type=1, head_dim=48, n_kv=65535, ctx=1 << 30)   # fp16: units of 32 rows
+    n = 1 << 20
+    a = _native.EhipAttend(q=P, out=P, q_stride=65535 * 48, out_stride=65535 * 48, n_tok=n, n_heads=65535, workspace=P, workspace_bytes=1 << 40)
+    assert L.ehip_attend(c, a, None) != 0 and "threads" in _native.last_error()
+
+
 def test_attend_workspace_covers_every_call():
     """No call of up to n tokens at any position asks for more than
     ehip_attend_workspace(n) (the refusal names what a call needs)."""
