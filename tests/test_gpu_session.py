@@ -3,6 +3,7 @@
 attention over it (ehip_attend), each against 64-bit references (session_ref),
 and a run of them together."""
 import ctypes
+import math
 import os
 import sys
 
@@ -495,6 +496,59 @@ def test_attend_strides_and_positions_of_many_rows(hd):
             check_attend(got[a:b], c, q[a:b], k, v, p + a)
         assert (got[:min(a, n)] == 0).all() and (got[max(b, 0):] == 0).all()
     R.hip().h.hipStreamDestroy(stream)
+
+
+@pytest.mark.parametrize("kind,hd", [(F32, 64), (F16, 128), (Q4, 128), (Q4, 64)])
+@pytest.mark.parametrize("step", [0.4, 1.9, 2.1, -1.5])
+@pytest.mark.parametrize("n,heads", [(1, 2), (40, 2), (48, 500)])
+def test_attend_a_rising_maximum(kind, hd, step, n, heads):
+    """Scores that rise from tile to tile by less and by more (in powers of
+    two) than the running maximum lags behind, or fall."""
+    rng = np.random.default_rng(n)
+    ctx = 400
+    k, v = kv_rows(rng, ctx, 1, hd)
+    v *= (1 + np.arange(ctx) % 7)[:, None, None].astype(np.float32)
+    k *= np.float32(0.1)
+    k[:, 0, 0] += (np.arange(ctx) // 32 * step).astype(np.float32)
+    q = rng.standard_normal((n, heads, hd)).astype(np.float32)
+    q[:, :, 0] = math.log(2) * math.sqrt(hd)
+    c = Cache(kind, 1, hd, ctx)
+    c.store(k, v, 0)
+    check_attend(attend(c, q, ctx - n), c, q, k, v, ctx - n)
+
+
+@pytest.mark.parametrize("kind,hd,n,heads", [(Q4, 128, 1, 2), (Q4, 128, 23, 4), (Q4, 64, 70, 14), (F16, 64, 9, 6), (F32, 64, 30, 6), (F32, 128, 40, 1300)])
+def test_captured_calls_on_two_streams(kind, hd, n, heads):
+    """Two captured calls with a workspace each, replayed at the same time on
+    two streams with eager calls between: every replay gives the eager rows."""
+    lib, h = _native.lib(), R.hip()
+    c, k, v, rng = filled(kind, hd, 2, 700, 700, n)
+    qs = [rng.standard_normal((n, heads, hd)).astype(np.float32) for _ in range(2)]
+    at = (700 - n, 411)
+    want = [attend(c, q, p) for q, p in zip(qs, at)]
+    check_attend(want[0], c, qs[0], k, v, at[0])
+    w = heads * hd
+    bufs, outs = [R.Buf(q) for q in qs], [R.Buf(np.zeros((n, w), np.float32)) for _ in qs]
+    spaces = [R.Buf(np.zeros(lib.ehip_attend_workspace(c.c, heads, n), np.uint8)) for _ in qs]
+    calls = [_native.EhipAttend(q=b.ptr, out=o.ptr, q_stride=w, out_stride=w, n_tok=n, n_heads=heads, pos0=p, workspace=s.ptr, workspace_bytes=s.nbytes)
+             for b, o, p, s in zip(bufs, outs, at, spaces)]
+    streams = [h.stream() for _ in qs]
+    made = [h.capture(s, lambda x=x, s=s: ok(lib.ehip_attend(c.c, x, s))) for x, s in zip(calls, streams)]
+    for _ in range(4):
+        for o in outs:
+            o.write(np.full((n, w), 7, np.float32))
+        for _ in range(3):
+            for (_, run), s in zip(made, streams):
+                assert h.h.hipGraphLaunch(run, s) == 0
+        for s in streams:
+            assert h.h.hipStreamSynchronize(s) == 0
+        for o, x in zip(outs, want):
+            np.testing.assert_array_equal(o.read().reshape(x.shape), x)
+        np.testing.assert_array_equal(attend(c, qs[0], at[0]), want[0])
+    for (graph, run), s in zip(made, streams):
+        h.h.hipGraphExecDestroy(run)
+        h.h.hipGraphDestroy(graph)
+        h.h.hipStreamDestroy(s)
 
 
 def test_attend_far_positions():
