@@ -37,6 +37,15 @@
 // NaN (infinite or NaN values, scales of positions never stored) a 4-bit scale
 // becomes zero and the scores of the rows that see it NaN, and an fp16 or fp32
 // value's products are made one by one for the rows that see it.
+//
+// Bound.  A token: the launch, its loads' latencies and, where ranges are joined,
+// a round trip past the L2 each for the partial rows, the count and the join (16
+// heads of 128 over 4 bits: 60 to 128 positions 5 us, 4096 10.4, 40,000 20.2 for
+// 46 MB).  A prompt: the vector units, which make codes into operands, halves
+// and exponentials (4 bits, 4096 tokens: 617 instructions a tile and wave, 73% of
+// the time; matrix cores 37%, 880 TFLOP/s of fp16 products) and, for fp16, the
+// loads' latencies (without them 186 us would be 135).  16 heads of 128 over 4
+// bits: 128 tokens 9 us, 512 16, 1024 27, 2048 70, 4096 196; fp16 4096 186.
 #include "attend.h"
 
 namespace ehip {
@@ -440,7 +449,7 @@ template <int HD, int CT, bool PACK, bool QL> struct Tile<EHIP_KV_F32, HD, CT, P
 // ---- the kernel ------------------------------------------------------------
 // Q in LDS, where the outputs go at the end, instead of in 64 registers: 32 rows
 // of 128 dims then leave room for two waves on a SIMD (16 heads of 128, 4096
-// tokens: 4 bits 305 -> 223 us, fp16 270 -> 211).  64 dims have two waves in
+// tokens: 4 bits 305 -> 223 us, fp16 270 -> 205).  64 dims have two waves in
 // any case (4 bits, 14 heads and 4096 tokens 115 -> 129), and an fp32 tile
 // would spill (1024 tokens 61 -> 105).
 constexpr bool q_in_lds(int type, int hd, int ct) { return type != EHIP_KV_F32 && hd == 128 && ct == 2; }
@@ -585,7 +594,7 @@ __global__ __launch_bounds__(64 * NW, 2) void k_attend_two(AttendArgs a) { atten
 // Rows of a unit: 8 (PACK) or 16 while they hold all the rows of a key head,
 // then 32; over an fp32 cache ATTEND_ROWS (attend_rows.hip), if that makes four
 // tiles and more for each workgroup that the GPU holds: 16 heads of 128, whole
-// prompts, 512 tokens 36 us (48 there), 1024 61 (64), 2048 183 (129).  Waves of
+// prompts, 512 tokens 27 us (48 there), 1024 61 (57), 2048 183 (120).  Waves of
 // a workgroup: 4; for few rows of a 4-bit cache 8 where 4 would make more
 // workgroups than CUs, as half the ranges are then joined (16 heads of 128 over
 // 8192 positions 15.0 -> 13.4 us; over 2048, which 4 waves spread over more

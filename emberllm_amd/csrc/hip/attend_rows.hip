@@ -7,7 +7,8 @@
 // of it, into LDS fragments that lie as the matrix cores' operands (64 lanes x
 // 16 bytes, so every read and write of a wave is 1 KB without bank conflicts):
 //   K   [hi, lo][half s][32 dims b]: lane (l, g) holds position 16 s + l, dims
-//       32 b + 8 g .. + 7
+//       32 b + 8 g .. + 7 (in the place of lane l ^ (g + 4 (b & 1)): eight lanes of
+//       a staging wave hold one position, whose pieces would share their banks)
 //   V   [hi, lo][16 dims d]: lane (l, g) holds dim 16 d + l, positions
 //       16 s + 4 g + i in the order (i, s) of the probabilities
 // while the next tile's rows are on their way to registers, and the tile after a
@@ -20,12 +21,13 @@
 // products on the fp16 matrix cores, which take sixteen times the fp32 ones' rate.
 //
 // Bound: the latencies of a wave's chain of products, maximum, exponentials and
-// halves, which two waves on a SIMD hide in part; not LDS and not the matrix
-// cores' rate.  Whole prompts, 16 heads over 8 of 128 dims: 1024 tokens 64 us
-// (attend.hip 61), 2048 129 (183), 4096 311 (637); 9 over 3 of 64: 1024 38 (35),
-// 2048 64 (78), 4096 148 (221).  A cache of 16 bits or 4 needs no splitting that
-// is worth a barrier: attend.hip is as fast there (4096 tokens 211 and 223 us at
-// 128 dims, where this kernel's form for them took 212 and 228).
+// halves, which two waves on a SIMD hide in part; the vector units issue 56% of
+// the time, the matrix cores work 32% of it.  Whole prompts, 16 heads over 8 of
+// 128 dims: 1024 tokens 57 us (attend.hip 61), 2048 120 (183), 4096 281 (637: 980
+// TFLOP/s of fp16 products for 489 of fp32); behind a window of 1024 with 4 sinks
+// 139; 9 over 3 of 64: 2048 62 (78), 4096 138 (221).  A cache of 16 bits or 4 needs
+// no splitting that is worth a barrier: attend.hip was as fast with them (4096
+// tokens 211 and 223 us at 128 dims, this kernel's form for them 212 and 228).
 #include "attend.h"
 
 namespace ehip {
@@ -116,8 +118,8 @@ template <int HD> struct Stager {
             }
             if (HD % 32 != 0 && 8 * p >= HD) hi = lo = i32x4{0, 0, 0, 0};   // (HD 48: the last fragment's upper half)
             if (HD % 64 == 0 || p < 4 * NB) {
-                o.k[0][s * NB + p / 4][(p % 4) * 16 + l] = hi;
-                o.k[1][s * NB + p / 4][(p % 4) * 16 + l] = lo;
+                o.k[0][s * NB + p / 4][(p % 4) * 16 + (l ^ (p & 7))] = hi;
+                o.k[1][s * NB + p / 4][(p % 4) * 16 + (l ^ (p & 7))] = lo;
             }
         }
         // ---- values
@@ -232,8 +234,9 @@ __global__ __launch_bounds__(64 * AR_NW, 2) void k_attend_rows(AttendArgs a) {
                 for (int c = 0; c < CT; c++) P[c][s] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
                 for (int b = 0; b < NB; b++) {
-                    const i32x4 kh = t.k[0][s * NB + b][lane];
-                    const i32x4 kl = t.k[1][s * NB + b][lane];
+                    const int at = lane ^ (g + 4 * (b & 1));
+                    const i32x4 kh = t.k[0][s * NB + b][at];
+                    const i32x4 kl = t.k[1][s * NB + b][at];
 #pragma unroll
                     for (int c = 0; c < CT; c++) {
                         P[c][s] = mfma16(kh, Q[c].q[b][1], P[c][s]);

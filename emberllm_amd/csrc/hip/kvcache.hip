@@ -13,7 +13,9 @@
 // Bound: memory.  A workgroup takes one tile of one key head: a thread's piece
 // of a row is 8 consecutive dims (its block's maximum over the 4 threads of the
 // block, a quad of lanes); values' codes then cross over through LDS, 8
-// positions of 8 dims at a time.
+// positions of 8 dims at a time.  8 heads of 128: a token 3.5 us (the launch and
+// three trips to memory), 4001 tokens 8.8 us (42 MB, 4.8 TB/s; a copy reaches
+// 4.9); the keys back as fp32 6.0 us, the values 6.9 (21 MB).
 #include "session.h"
 
 namespace ehip {

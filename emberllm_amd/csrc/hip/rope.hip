@@ -14,7 +14,10 @@
 //
 // Bound: memory (4 bytes in and out per value).  A wave takes one token and
 // the heads of one part of its row; a lane holds VEC dims and their partners,
-// computes their VEC angles once and uses them for all of its heads.
+// computes their VEC angles once and uses them for all of its heads.  A token of
+// 16 + 8 heads of 128 with QK-norm 3.4 us (the launch); 4096 tokens of 9 + 3 heads
+// of 64, half of each turning, 7.3 us (25 MB, 3.4 TB/s at this length, start and
+// end included).
 #include <cmath>
 
 #include "session.h"
