@@ -23,8 +23,8 @@
 // Bound: the latencies of a wave's chain of products, maximum, exponentials and
 // halves, which two waves on a SIMD hide in part; the vector units issue 56% of
 // the time, the matrix cores work 32% of it.  Whole prompts, 16 heads over 8 of
-// 128 dims: 1024 tokens 57 us (attend.hip 61), 2048 120 (183), 4096 281 (637: 980
-// TFLOP/s of fp16 products for 489 of fp32); behind a window of 1024 with 4 sinks
+// 128 dims: 1024 tokens 57 us (attend.hip 61), 2048 120 (183), 4096 281 (637: 245
+// TFLOP/s of fp32 work, 734 of fp16 products); behind a window of 1024 with 4 sinks
 // 139; 9 over 3 of 64: 2048 62 (78), 4096 138 (221).  A cache of 16 bits or 4 needs
 // no splitting that is worth a barrier: attend.hip was as fast with them (4096
 // tokens 211 and 223 us at 128 dims, this kernel's form for them 212 and 228).
