@@ -551,6 +551,17 @@ def test_captured_calls_on_two_streams(kind, hd, n, heads):
         h.h.hipStreamDestroy(s)
 
 
+@pytest.mark.parametrize("kind,hd", KINDS)
+def test_attend_long_caches(kind, hd):
+    """Units of 8, 16 and 32 rows over 20,000 positions (many tiles to a wave,
+    workgroups of eight waves over 4 bits), whole and behind a window."""
+    c, k, v, rng = filled(kind, hd, 2, 20011, 20032, 3)
+    for n, G in ((1, 2), (2, 4), (1, 12), (2, 8), (3, 7)):
+        q = rng.standard_normal((n, 2 * G, hd)).astype(np.float32)
+        check_attend(attend(c, q, 20011 - n), c, q, k, v, 20011 - n)
+        check_attend(attend(c, q, 20011 - n, 9000, 70), c, q, k, v, 20011 - n, 9000, 70)
+
+
 def test_attend_far_positions():
     """A token at the end of a long cache: 40,000 positions in 4 bits, and fp16
     rows whose offsets pass 2^31 bytes."""
