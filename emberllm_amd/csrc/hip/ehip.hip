@@ -868,11 +868,10 @@ static int enq_session_attn(EhipState *s, int l, float *qkv, int n, int pos0, co
     r.x = qkv; r.out = qkv; r.x_stride = r.out_stride = stride;
     r.n_tok = n; r.n_q = c.n_heads; r.n_k = c.n_kv_heads; r.pos0 = pos0; r.pos = pos;
     r.q_norm = y.q_norm; r.k_norm = y.k_norm; r.eps = c.norm_eps;
-    if (launch_rope(s->st, s->plan, r)) return -1;
     const EhipCache k = layer_cache(s, l);
     EhipCacheRows w{};
     w.k = qkv + qd; w.v = qkv + qd + kvd; w.k_stride = w.v_stride = stride; w.n_tok = n; w.pos0 = pos0; w.pos = pos;
-    if (launch_cache_store(s->st, k, w)) return -1;
+    if (n == 1 ? launch_rope_store(s->st, s->plan, r, k, w) : launch_rope(s->st, s->plan, r) || launch_cache_store(s->st, k, w)) return -1;
     EhipAttend a{};
     a.q = qkv; a.out = out; a.q_stride = stride; a.out_stride = qd;
     a.n_tok = n; a.n_heads = c.n_heads; a.pos0 = pos0; a.pos = pos; a.window = s->window; a.sinks = s->sinks;

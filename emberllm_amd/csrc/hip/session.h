@@ -36,6 +36,7 @@ __host__ __device__ constexpr int kv_scale_at(int hd, int g, int b, int i, int s
 
 int launch_rope(hipStream_t st, const EhipRopePlan &p, const EhipRopeRows &r);
 int launch_cache_store(hipStream_t st, const EhipCache &c, const EhipCacheRows &r);
+int launch_rope_store(hipStream_t st, const EhipRopePlan &p, const EhipRopeRows &r, const EhipCache &c, const EhipCacheRows &w);   // one token
 int launch_attend(hipStream_t st, const EhipCache &c, const EhipAttend &q);   // sets ehip_last_error() itself
 
 // 0, or -1 with ehip_last_error() set: a cache that the kernels support

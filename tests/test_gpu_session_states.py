@@ -77,7 +77,8 @@ def check_layer(eng, cfg, rc, layer, qkv, o, pos0, window, sinks):
 CASES = [("t_llama", "f32", 0, 0, None), ("t_gqa", "q4", 20, 3, None), ("t_qwen3", "f16", 0, 0, dict(scaling=3, factor=4.0, orig_ctx=96)),
          ("t_qwen3", "q4", 0, 0, None), ("t_f32", "f32", 16, 1, dict(rotary_dim=24)), ("t_f32", "f16", 0, 0, dict(scaling=1, factor=2.0)),
          ("t_bias", "q4", 33, 0, dict(scaling=4, factor=8.0, orig_ctx=64)), ("t_g7", "q4", 100, 5, dict(rotary_dim=32, scaling=2, factor=2.0)),
-         ("w64", "q4", 64, 4, None), ("w128", "q4", 0, 0, dict(scaling=3, factor=2.0, orig_ctx=400)), ("w128", "f32", 40, 2, None)]
+         ("w64", "q4", 64, 4, None), ("w128", "q4", 0, 0, dict(scaling=3, factor=2.0, orig_ctx=400)), ("w128", "f32", 40, 2, None),
+         ("t_gqa", "q4", 0, 0, dict(rotary_dim=20)), ("t_qwen3", "f16", 30, 2, dict(rotary_dim=10)), ("t_f32", "f32", 0, 0, dict(rotary_dim=14))]
 
 
 @pytest.mark.parametrize("name,kv,window,sinks,scaled", CASES)
